@@ -367,6 +367,95 @@ q3_status q3_gemm_f16(void* out, const uint16_t* a, const uint16_t* w, const uin
  * to *out_index (device int32). n == 0 is rejected like the reference's empty span. */
 q3_status q3_greedy(const float* logits, int n, int32_t* out_index, void* stream);
 
+/* ------------------------------------------------------------------ paged KV pools
+ * Serving operators over a caller-owned paged cache (no counterpart in the reference, whose KVCache
+ * is one contiguous bf16 array per layer, include/inference.h:140-161): rows quantised as they are
+ * written and read back, attention over them with or without a prefix that all sequences share, and
+ * the acceptance of drafted tokens. As the free kernels above they take device pointers, are
+ * enqueued on `stream`, return after enqueueing, allocate nothing, keep nothing from one call for
+ * the next and can be captured into a CUDA graph (the host arguments are then fixed; lengths, tables
+ * and slots are read on the device at every replay). Every pointer has to be memory of one device;
+ * that device need not be the current one, and `stream` belongs to it.
+ *
+ * A pool has 16-token pages, per page n_kv_heads x 16 rows of head_dim (64 or 128) values, for K and
+ * for V: the layout of a model's own cache. Slot s is row s % 16 of page s / 16. type Q3_TYPE_BF16:
+ * bf16 bits, exps NULL. type Q3_TYPE_E4M3: one byte a value (4 significant bits against bf16's 8,
+ * half the bytes), and each row of K and of V has one power of two: exps[page][head][16][2] bytes,
+ * K's and V's, and the value is code * 2^(byte - 127). k and v are 16-byte aligned, exps 4-byte. */
+enum { Q3_TYPE_F32 = 0, Q3_TYPE_BF16 = 1, Q3_TYPE_F16 = 2, Q3_TYPE_E4M3 = 3 };
+typedef struct q3_kv_pool {
+    void* k;
+    void* v;
+    uint8_t* exps;
+    int64_t n_pages; /* at most 2^27 - 1: slots are int32 */
+    int32_t n_kv_heads, head_dim, type;
+} q3_kv_pool;
+
+/* Writes n tokens' K and V rows: token i's n_kv_heads * head_dim values (type F32, BF16 or F16) start
+ * at element i * k_stride of k (i * v_stride of v) and go to slot slots[i]; a slot that is negative
+ * or past the pool's end is skipped (the padding of a batch). An e4m3 row's byte is the smallest in
+ * [0, 254] for which the row's largest finite magnitude is at most 448 * 2^(byte - 127), so scaling
+ * is exact and each value is rounded once, to nearest even; infinities become +-448 * 2^(byte - 127),
+ * NaN stays NaN. The slots of one call are distinct (where two rows name one slot, its bytes may
+ * come from either). */
+q3_status q3_kv_write(const q3_kv_pool* pool, const void* k, const void* v, int type,
+                      int64_t k_stride, int64_t v_stride, const int32_t* slots, int n, void* stream);
+/* Reads n slots back, laid out as q3_kv_write takes them, in `type` (rounded to nearest even; F16
+ * overflows to infinity). A slot that is negative or past the pool's end reads as zeros. */
+q3_status q3_kv_read(const q3_kv_pool* pool, void* k, void* v, int type, int64_t k_stride,
+                     int64_t v_stride, const int32_t* slots, int n, void* stream);
+
+/* FastAttn (src/inference.cpp:1017-1058) of a ragged batch's newest rows over a paged pool: sequence
+ * b has query rows q_start[b] .. q_start[b+1]-1 (at most max_q; q_start[0] >= 0, ascending, at most
+ * n_q) and kv_len[b] cached tokens, its rows being the last of them: row i of its n_b sees tokens
+ * 0 .. kv_len[b] - n_b + i. One row a sequence is a decode step, more are drafted tokens. Token t of
+ * sequence b lies in page table[b * table_stride + t / 16]; kv_len[b] is at most 16 * table_stride. A
+ * table entry outside the pool takes its 16 tokens out of the attention. A row that sees nothing is
+ * zeros. Rows that belong to no sequence are left as they were.
+ * q and out: rows of n_heads heads of head_dim values, q_stride / out_stride elements apart, type BF16
+ * (either pool) or F16 (an e4m3 pool), 16-byte aligned; n_heads a multiple of pool->n_kv_heads, at
+ * most 64 query heads per KV head; scores are divided by sqrt(head_dim). max_q * n_heads /
+ * n_kv_heads is at most 128. workspace: q3_paged_attn_workspace_size bytes (prefix_len 0), 16-byte
+ * aligned, used by one call at a time. Sums and softmax statistics are fp32; the probabilities are
+ * rounded to fp16 for an e4m3 pool, split into two bf16 values for a bf16 one. */
+size_t q3_paged_attn_workspace_size(const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs,
+                                    int max_q, int prefix_len);
+q3_status q3_paged_attn(void* out, void* workspace, const void* q, int type, int64_t q_stride,
+                        int64_t out_stride, const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs,
+                        int max_q, const int32_t* q_start, const int32_t* kv_len,
+                        const int32_t* table, int table_stride, void* stream);
+/* q3_paged_attn where the prefix_len tokens of prefix_table's pages come before every sequence's own
+ * tokens and are seen by every row: their keys are read once for the rows of all sequences, as
+ * tensor-core contractions (tcgen05), and joined with each sequence's own part by the softmax
+ * statistics. prefix_len may be any number (the last page need not be full); kv_len counts a
+ * sequence's own tokens alone and may be 0. The workspace is sized with this prefix_len. A
+ * tensor-core pipeline wait that gives up (it is bounded) leaves NaN in the rows of its part. */
+q3_status q3_prefix_attn(void* out, void* workspace, const void* q, int type, int64_t q_stride,
+                         int64_t out_stride, const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs,
+                         int max_q, const int32_t* q_start, const int32_t* kv_len,
+                         const int32_t* table, int table_stride, const int32_t* prefix_table,
+                         int prefix_len, void* stream);
+
+/* Speculative sampling's acceptance, beside Sampler::Greedy (src/inference.cpp:703-709): sequence b
+ * has n_drafts[b] drafted tokens draft_tokens[b * max_drafts + j] (n_drafts NULL: max_drafts each),
+ * the target's probabilities before each and after the last, target[b * t_seq + j * t_row + token],
+ * and those they were drawn from, draft[b * d_seq + j * d_row + token] (NULL: each draft was certain,
+ * probability 1 for its token and 0 elsewhere). Draft j is accepted while
+ * u_accept[b * max_drafts + j] * draft(token) < target(token). After the first rejection the next
+ * token is drawn from max(target - draft, 0) of that position, after no rejection from the target's
+ * last row: with C the running sum over the vocabulary, the first token with C > u_sample[b] * C_last
+ * (where no token reaches it, u_sample = 1 for instance, the last with a positive share); a residual without a
+ * positive share gives way to the target's row, and that without one to token 0. Products, differences and sums are in 64 bits,
+ * so the token does not depend on their order. A draft outside the vocabulary is rejected, and NaN
+ * counts as 0. tokens[b * (max_drafts + 1) + ..] receives the accepted drafts, the drawn token and -1
+ * for the rest, n_accepted[b] the number of accepted drafts. Numbers u are in [0, 1). With
+ * max_drafts 0 draft, draft_tokens and u_accept are not read. */
+q3_status q3_verify_drafts(int32_t* tokens, int32_t* n_accepted, const float* target, int64_t t_seq,
+                           int64_t t_row, const float* draft, int64_t d_seq, int64_t d_row,
+                           const int32_t* draft_tokens, const int32_t* n_drafts,
+                           const float* u_accept, const float* u_sample, int n_seqs, int max_drafts,
+                           int vocab, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

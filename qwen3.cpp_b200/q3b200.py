@@ -75,6 +75,13 @@ class GenStats(C.Structure):
                 ("stopped_on_eos", C.c_int32), ("reached_token_limit", C.c_int32)]
 
 
+class KvPool(C.Structure):
+    """A caller-owned paged KV pool on device pointers (q3_kv_pool): KvPool(k, v, exps, n_pages,
+    n_kv_heads, head_dim, type), exps None for TYPE_BF16."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("exps", C.c_void_p), ("n_pages", C.c_int64),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("type", C.c_int32)]
+
+
 _lib = None
 
 
@@ -87,7 +94,8 @@ def lib() -> C.CDLL:
         raise FileNotFoundError(
             f"{LIB_PATH} is missing: build it with `python qwen3.cpp_b200/build.py`")
     L = C.CDLL(str(LIB_PATH))
-    vp, i32, sz = C.c_void_p, C.c_int32, C.c_size_t
+    vp, i32, sz, i64 = C.c_void_p, C.c_int32, C.c_size_t, C.c_int64
+    pool = C.POINTER(KvPool)
     L.q3_last_error.restype = C.c_char_p
     L.q3_version.restype = C.c_char_p
     sig = {
@@ -151,6 +159,14 @@ def lib() -> C.CDLL:
         "q3_attn": [vp, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp],
         "q3_attn_noalloc": [vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp],
         "q3_greedy": [vp, C.c_int, vp, vp],
+        "q3_kv_write": [pool, vp, vp, C.c_int, i64, i64, vp, C.c_int, vp],
+        "q3_kv_read": [pool, vp, vp, C.c_int, i64, i64, vp, C.c_int, vp],
+        "q3_paged_attn": [vp, vp, vp, C.c_int, i64, i64, pool, C.c_int, C.c_int, C.c_int, C.c_int,
+                          vp, vp, vp, C.c_int, vp],
+        "q3_prefix_attn": [vp, vp, vp, C.c_int, i64, i64, pool, C.c_int, C.c_int, C.c_int, C.c_int,
+                           vp, vp, vp, C.c_int, vp, C.c_int, vp],
+        "q3_verify_drafts": [vp, vp, vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, C.c_int, C.c_int,
+                             C.c_int, vp],
     }
     for name, args in sig.items():
         f = getattr(L, name)
@@ -166,6 +182,8 @@ def lib() -> C.CDLL:
     L.q3_tp_free.restype = None
     L.q3_attn_workspace_size.argtypes = [C.c_int, C.c_int]
     L.q3_attn_workspace_size.restype = sz
+    L.q3_paged_attn_workspace_size.argtypes = [pool] + [C.c_int] * 5
+    L.q3_paged_attn_workspace_size.restype = sz
     L.q3_attn_noalloc_max_scratch.argtypes = []
     L.q3_attn_noalloc_max_scratch.restype = sz
     _lib = L
@@ -615,3 +633,49 @@ def gemm_bf16(out: int, a: int, w: int, w3, M: int, N: int, K: int, epilogue: in
 def gemm_f16(out: int, a: int, w: int, w3, M: int, N: int, K: int, epilogue: int, stream=None):
     """q3_gemm_f16: as gemm_bf16 with fp16 operands (and fp16 SwiGLU / 16-bit stores)."""
     check(lib().q3_gemm_f16(out, a, w, w3, M, N, K, epilogue, stream))
+
+
+# ------------------------------------------------------------------ paged KV pools (device pointers)
+
+TYPE_F32, TYPE_BF16, TYPE_F16, TYPE_E4M3 = 0, 1, 2, 3
+
+
+def kv_write(pool: KvPool, k, v, type: int, k_stride: int, v_stride: int, slots, n: int, stream=None):
+    """q3_kv_write: n tokens' K and V rows into the pool's slots, quantised for a TYPE_E4M3 pool."""
+    check(lib().q3_kv_write(pool, k, v, type, k_stride, v_stride, slots, n, stream))
+
+
+def kv_read(pool: KvPool, k, v, type: int, k_stride: int, v_stride: int, slots, n: int, stream=None):
+    """q3_kv_read: n slots' K and V rows of the pool, in `type`."""
+    check(lib().q3_kv_read(pool, k, v, type, k_stride, v_stride, slots, n, stream))
+
+
+def paged_attn_workspace_size(pool: KvPool, n_heads: int, n_q: int, n_seqs: int, max_q: int,
+                              prefix_len: int = 0) -> int:
+    return int(lib().q3_paged_attn_workspace_size(pool, n_heads, n_q, n_seqs, max_q, prefix_len))
+
+
+def paged_attn(out, ws, q, type: int, q_stride: int, out_stride: int, pool: KvPool, n_heads: int,
+               n_q: int, n_seqs: int, max_q: int, q_start, kv_len, table, table_stride: int,
+               stream=None):
+    """q3_paged_attn: each sequence's newest rows over its own pages."""
+    check(lib().q3_paged_attn(out, ws, q, type, q_stride, out_stride, pool, n_heads, n_q, n_seqs,
+                              max_q, q_start, kv_len, table, table_stride, stream))
+
+
+def prefix_attn(out, ws, q, type: int, q_stride: int, out_stride: int, pool: KvPool, n_heads: int,
+                n_q: int, n_seqs: int, max_q: int, q_start, kv_len, table, table_stride: int,
+                prefix_table, prefix_len: int, stream=None):
+    """q3_prefix_attn: as paged_attn behind a prefix that every sequence shares."""
+    check(lib().q3_prefix_attn(out, ws, q, type, q_stride, out_stride, pool, n_heads, n_q, n_seqs,
+                               max_q, q_start, kv_len, table, table_stride, prefix_table,
+                               prefix_len, stream))
+
+
+def verify_drafts(tokens, n_accepted, target, t_seq: int, t_row: int, draft, d_seq: int, d_row: int,
+                  draft_tokens, n_drafts, u_accept, u_sample, n_seqs: int, max_drafts: int,
+                  vocab: int, stream=None):
+    """q3_verify_drafts: the accepted drafts of every sequence and the token drawn after them."""
+    check(lib().q3_verify_drafts(tokens, n_accepted, target, t_seq, t_row, draft, d_seq, d_row,
+                                 draft_tokens, n_drafts, u_accept, u_sample, n_seqs, max_drafts,
+                                 vocab, stream))
