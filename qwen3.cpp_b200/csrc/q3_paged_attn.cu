@@ -1,26 +1,669 @@
 // q3_paged_attn / q3_prefix_attn: attention of a ragged batch's newest rows over a paged KV pool,
 // with or without a prefix that every sequence shares.
+//
+// own_pages_kernel computes the part over each sequence's own pages, join_kernel joins the parts.
+//
+// Work: a unit is one page of one (sequence, KV head, group of 8 * NT rows). The units of all
+// sequences form one line, cut into equal runs, one a block, so a ragged batch loads every block
+// alike and a long sequence spreads over many. Each block finds its run from the lengths on the
+// device (a scan over the sequences), so a captured graph follows them. A (sequence, head, group)
+// inside one run is finished there; one that is cut leaves a part per block, at most two a block, and
+// join_kernel adds them by their softmax statistics.
+//
+// A block's four warps take every fourth page. A page is 16 keys, one m16n8k16 operand tile:
+//   S^T[16 keys x 8 rows] = K . Q^T      K's rows are the A operand as they lie in memory
+//   O^T[d x 8 rows]      += V^T . P^T    two keys' V values of one d are a register of A
+// The order of the head's dimensions inside an operand is free as long as both sides agree, so a lane
+// loads 16 contiguous bytes and they are its operand registers (bf16) or become them by a conversion
+// (e4m3 -> fp16, exact); V pairs need one byte permutation. Nothing goes through shared memory: K of
+// page i + 4 is on its way while the scores of page i turn into weights, V while its K is multiplied.
+// The scores come out transposed for the second product; movmatrix turns the rounded weights.
+//
+// The running maximum moves only when a score passes it by more than 2^4 (one vote a page instead of
+// two times three shuffles): weights are then at most 2^(kShift + 4), which fp16 holds, as it does 2^3
+// more for V rows' own powers of two, whose running maximum is treated alike.
+//
+// Rounding: e4m3 -> fp16 is exact; a query row is scaled by a power of two so that its largest value
+// is in [2^13, 2^14): bf16 and fp16 values are then fp16 values down to 2^-38 of the row's largest.
+// Weights are rounded to fp16 (2^-11), for a bf16 pool to a bf16 pair hi + lo (2^-16). Sums are fp32.
+//
+// Bound by HBM: 2 * (D + 1) bytes a key and KV head (e4m3).
+#include <algorithm>
 #include <climits>
 
-#include "q3_paged.cuh"
+#include "q3_paged_attn.cuh"
 
 namespace q3 {
 
 namespace {
 
-struct PagedArgs {
-    void* out;
-    const void* q;
-    const void* k;
-    const void* v;
-    const uint8_t* exps;
-    const int32_t* q_start;
-    const int32_t* kv_len;
-    const int32_t* table;
-    const int32_t* prefix_table;
-    long long q_stride, out_stride;
-    int n_pages, n_kv, group, n_q, n_seqs, max_q, table_stride, prefix_len, f16, e4m3;
-};
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr float kGrow = 4.0f;  // how far (log2) a score may pass the running maximum
+constexpr int kGrowV = 3;      // the same for V's powers of two
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (F16) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    } else {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* r) {
+    static_assert(BYTES == 8 || BYTES % 16 == 0, "run width");
+    if constexpr (BYTES == 8) {
+        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+    } else {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) {
+            const uint4 x = ldg_stream(p + 16 * i);
+            r[4 * i] = x.x;
+            r[4 * i + 1] = x.y;
+            r[4 * i + 2] = x.z;
+            r[4 * i + 3] = x.w;
+        }
+    }
+}
+
+// Whether a packed word of pool values holds an infinity or NaN.
+template <bool E4M3>
+__device__ __forceinline__ bool odd_word(uint32_t x) {
+    return E4M3 ? (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0
+                : (((x & 0x7fff7fffu) + 0x00800080u) & 0x80008000u) != 0;
+}
+
+// The A operand of O^T += V^T P^T for m-tile i: a0, a1 from the keys 2t, 2t + 1, a2, a3 from 2t + 8,
+// 2t + 9 (t = lane % 4), for the lane's values 2i and 2i + 1 of each.
+template <bool E4M3, int VW>
+__device__ __forceinline__ void v_operand(const uint32_t (&vr)[4][VW], int i, uint32_t (&f)[4]) {
+    if constexpr (E4M3) {
+        const uint32_t sel = i & 1 ? 0x7362u : 0x5140u;
+        const uint32_t p0 = __byte_perm(vr[0][i >> 1], vr[1][i >> 1], sel);
+        const uint32_t p1 = __byte_perm(vr[2][i >> 1], vr[3][i >> 1], sel);
+        f[0] = e4m3x2_to_f16x2(p0);
+        f[1] = e4m3x2_hi_to_f16x2(p0);
+        f[2] = e4m3x2_to_f16x2(p1);
+        f[3] = e4m3x2_hi_to_f16x2(p1);
+    } else {
+        f[0] = __byte_perm(vr[0][i], vr[1][i], 0x5410u);
+        f[1] = __byte_perm(vr[0][i], vr[1][i], 0x7632u);
+        f[2] = __byte_perm(vr[2][i], vr[3][i], 0x5410u);
+        f[3] = __byte_perm(vr[2][i], vr[3][i], 0x7632u);
+    }
+}
+
+// Threads' sums of units, one after the other: the sums before this thread and of all.
+__device__ __forceinline__ void block_scan(long long mine, long long* warp_sums, long long& before,
+                                           long long& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    before = x - mine;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += warp_sums[w];
+        total += warp_sums[w];
+    }
+}
+
+template <int NT>
+__device__ __forceinline__ int row_groups(const SeqShape& s, int group) {
+    return (s.rows * group + 8 * NT - 1) / (8 * NT);
+}
+
+template <int D, bool E4M3, int NT>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2))
+    own_pages_kernel(const PagedArgs a) {
+    constexpr int MT = D / 16;                    // m-tiles of O^T, k-steps of S^T
+    constexpr int KW = E4M3 ? D / 16 : D / 8;     // words a lane holds of one K row
+    constexpr int VW = E4M3 ? D / 32 : D / 16;    // and of one V row
+    constexpr int ROW = E4M3 ? D : 2 * D;         // bytes of a pool row
+    constexpr int ROWS = 8 * NT;
+    __shared__ float o_s[kWarps][ROWS][D];
+    __shared__ float m_s[kWarps][ROWS], l_s[kWarps][ROWS];
+    __shared__ long long scan_s[kWarps];
+    __shared__ long long first_s;
+    __shared__ int seq_s;
+
+    pdl_trigger();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+
+    // This block's run of units.
+    const int per_thread = (a.n_seqs + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per_thread, a.n_seqs), b1 = min(b0 + per_thread, a.n_seqs);
+    auto units = [&](int b) {
+        const SeqShape s = seq_shape(a, b);
+        return static_cast<long long>(a.n_kv) * row_groups<NT>(s, a.group) * seq_pages(s);
+    };
+    long long mine = 0, before, total;
+    for (int b = b0; b < b1; ++b) mine += units(b);
+    block_scan(mine, scan_s, before, total);
+    const long long per = max(static_cast<long long>(kMinPages),
+                              (total + gridDim.x - 1) / static_cast<long long>(gridDim.x));
+    const long long start = per * blockIdx.x, end = min(total, start + per);
+    if (blockIdx.x == 0) {
+        long long x = before;
+        for (int b = b0; b < b1; ++b) {
+            a.first_unit[b] = x;
+            x += units(b);
+        }
+        if (tid == 0) {
+            a.first_unit[a.n_seqs] = total;
+            a.first_unit[a.n_seqs + 1] = per;
+        }
+    }
+    if (start >= end) return;
+    if (before <= start && start < before + mine) {
+        long long x = before;
+        int b = b0;
+        for (long long u; x + (u = units(b)) <= start; ++b) x += u;
+        seq_s = b;
+        first_s = x;
+    }
+    __syncthreads();
+
+    const uint8_t* kp = static_cast<const uint8_t*>(a.k);
+    const uint8_t* vp = static_cast<const uint8_t*>(a.v);
+    const float scale = 1.4426950408889634f / sqrtf(static_cast<float>(D));
+    long long pos = start, seq_first = first_s;
+    int b = seq_s;
+    while (pos < end) {
+        const SeqShape s = seq_shape(a, b);
+        const int pages = seq_pages(s), groups = row_groups<NT>(s, a.group);
+        const long long all = static_cast<long long>(a.n_kv) * groups * pages;
+        if (pos >= seq_first + all) {
+            seq_first += all;
+            ++b;
+            continue;
+        }
+        const long long strip = (pos - seq_first) / pages;  // (head, row group)
+        const int p0 = static_cast<int>(pos - seq_first - strip * pages);
+        const int p1 = static_cast<int>(min(static_cast<long long>(pages), p0 + (end - pos)));
+        const int h = static_cast<int>(strip / groups), rg = static_cast<int>(strip % groups);
+        const int r_base = rg * ROWS;
+        const int n_rows = min(ROWS, s.rows * a.group - r_base);
+
+        // Q as the B operand: lane (g, t) holds row g's values in the order of K's.
+        uint32_t qw[NT][D / 8];
+        float c_col[NT][2];  // score factor of the columns 2t, 2t + 1
+        int seen[NT][2];     // keys that they see
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = r_base + n * 8 + g;
+            const bool live = n * 8 + g < n_rows;
+            const uint16_t* qp = static_cast<const uint16_t*>(a.q) +
+                                 (live ? (s.row0 + r / a.group) * a.q_stride + (h * a.group + r % a.group) * D : 0);
+            constexpr int CH = E4M3 ? 16 : 8;  // consecutive values
+#pragma unroll
+            for (int j = 0; j < D / (4 * CH); ++j) {
+#pragma unroll
+                for (int i = 0; i < CH / 8; ++i) {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (live) x = *reinterpret_cast<const uint4*>(qp + j * 4 * CH + t * CH + 8 * i);
+                    uint32_t* w = &qw[n][(j * (CH / 8) + i) * 4];
+                    w[0] = x.x;
+                    w[1] = x.y;
+                    w[2] = x.z;
+                    w[3] = x.w;
+                }
+            }
+            float c = scale;
+            if constexpr (E4M3) {
+                float big = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const float lo = a.f16 ? f16_lo(qw[n][i]) : bf16_lo(qw[n][i]);
+                    const float hi = a.f16 ? f16_hi(qw[n][i]) : bf16_hi(qw[n][i]);
+                    big = fmaxf(big, fmaxf(fabsf(lo), fabsf(hi)));
+                }
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                int e = 0;
+                if (big > 0.0f && big < INFINITY) {
+                    e = min(13 + 127 - static_cast<int>(__float_as_uint(big) >> 23), 126);
+                }
+                const float f = pow2(e);
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const float lo = a.f16 ? f16_lo(qw[n][i]) : bf16_lo(qw[n][i]);
+                    const float hi = a.f16 ? f16_hi(qw[n][i]) : bf16_hi(qw[n][i]);
+                    qw[n][i] = pack2_out(lo * f, hi * f, 1);
+                }
+                c = scale * pow2(-e);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int rr = n * 8 + 2 * t + x;
+                c_col[n][x] = __shfl_sync(0xffffffffu, c, (2 * t + x) * 4);
+                seen[n][x] = rr < n_rows ? s.len - s.rows + (r_base + rr) / a.group + 1 : 0;
+            }
+        }
+        const int tail_key = s.len - s.rows + r_base / a.group + 1;  // seen by every row below it
+
+        float m[NT][2], neg[NT][2], l[NT][2], o[NT][MT][4];
+        int r_v = -1000;  // power of two that o is relative to
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                m[n][x] = -INFINITY;
+                neg[n][x] = kShift;
+                l[n][x] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+        }
+
+        const int32_t* table = a.table + static_cast<size_t>(b) * a.table_stride;
+        const int steps = p1 - p0 > warp ? (p1 - p0 - warp + kWarps - 1) / kWarps : 0;
+        int ids = 0;
+        auto page_of = [&](int it) {  // page of this warp's step `it` (in order: 0, 1, 2, ...)
+            if ((it & 31) == 0) {
+                const int p = p0 + warp + (it + lane) * kWarps;
+                ids = p < p1 ? table[p] : -1;
+            }
+            return __shfl_sync(0xffffffffu, ids, it & 31);
+        };
+        uint32_t kr[2][KW], vr[4][VW];
+        uint32_t ex[2] = {0, 0};
+        auto load_k = [&](int page) {
+            const size_t row = (static_cast<size_t>(page) * a.n_kv + h) * kPageTokens;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const uint8_t* p = kp + (row + g + 8 * x) * ROW + t * 16;
+#pragma unroll
+                for (int j = 0; j < KW / 4; ++j) load_bytes<16>(p + j * 64, &kr[x][4 * j]);
+            }
+        };
+        auto load_v = [&](int page) {
+            const size_t row = (static_cast<size_t>(page) * a.n_kv + h) * kPageTokens;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint8_t* p = vp + (row + 2 * t + (x & 1) + 8 * (x >> 1)) * ROW;
+                if constexpr (E4M3) {
+                    load_bytes<VW * 4>(p + g * (VW * 4), vr[x]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VW / 4; ++j) load_bytes<16>(p + j * 128 + g * 16, &vr[x][4 * j]);
+                }
+            }
+        };
+        auto load_exps = [&](int page, uint32_t (&to)[2]) {
+            if constexpr (E4M3) {
+                const uint16_t* p = reinterpret_cast<const uint16_t*>(a.exps) +
+                                    (static_cast<size_t>(page) * a.n_kv + h) * kPageTokens + g;
+                to[0] = __ldg(p);
+                to[1] = __ldg(p + 8);
+            }
+        };
+
+        int page = -1;
+        if (steps > 0) {
+            page = page_of(0);
+            const int safe = page >= 0 && page < a.n_pages ? page : 0;
+            load_k(safe);
+            load_exps(safe, ex);
+            load_v(safe);
+        }
+        for (int it = 0; it < steps; ++it) {
+            const int key0 = (p0 + warp + it * kWarps) * kPageTokens;
+            const bool there = page >= 0 && page < a.n_pages;
+            // Scores: two chains of products, so that one is not a wait for the other.
+            float sc[NT][2][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[n][0][i] = sc[n][1][i] = 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < MT; ++k) {
+                uint32_t f[4];
+                if constexpr (E4M3) {
+                    f[0] = e4m3x2_to_f16x2(kr[0][k]);
+                    f[1] = e4m3x2_to_f16x2(kr[1][k]);
+                    f[2] = e4m3x2_hi_to_f16x2(kr[0][k]);
+                    f[3] = e4m3x2_hi_to_f16x2(kr[1][k]);
+                } else {
+                    f[0] = kr[0][2 * k];
+                    f[1] = kr[1][2 * k];
+                    f[2] = kr[0][2 * k + 1];
+                    f[3] = kr[1][2 * k + 1];
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma16816<E4M3>(sc[n][k & 1], f[0], f[1], f[2], f[3], qw[n][2 * k], qw[n][2 * k + 1]);
+                }
+            }
+            int next = -1, next_safe = 0;
+            uint32_t ex_next[2] = {0, 0};
+            if (it + 1 < steps) {
+                next = page_of(it + 1);
+                next_safe = next >= 0 && next < a.n_pages ? next : 0;
+                load_k(next_safe);
+                load_exps(next_safe, ex_next);
+            }
+            const bool tail = !there || key0 + kPageTokens > tail_key;
+            const int limit = there ? s.len - key0 : 0;  // this page's keys that exist
+            float p[NT][4];
+            bool grow = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x = (sc[n][0][i] + sc[n][1][i]) * c_col[n][i & 1];
+                    if constexpr (E4M3) x *= __uint_as_float((ex[i >> 1] & 0xffu) << 23);  // 2^(byte - 127)
+                    if (tail && (!there || key0 + g + 8 * (i >> 1) >= seen[n][i & 1])) x = -INFINITY;
+                    p[n][i] = x;
+                    grow |= x > m[n][i & 1] + kGrow;
+                }
+            }
+            int v_top = 0;
+            if constexpr (E4M3) {
+                // A byte of a key that is not there says nothing.
+                const int e0 = g < limit ? ex[0] >> 8 : 0, e1 = g + 8 < limit ? ex[1] >> 8 : 0;
+                v_top = max(e0, e1);
+                grow |= v_top > r_v + kGrowV;
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+                float fv = 1.0f;
+                if constexpr (E4M3) {
+                    const int r_new = max(r_v, static_cast<int>(__reduce_max_sync(0xffffffffu, v_top)));
+                    fv = pow2(r_v - r_new);
+                    r_v = r_new;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float f[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float mx = fmaxf(p[n][x], p[n][x + 2]);
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        const float m_new = fmaxf(m[n][x], mx);
+                        f[x] = m_new == m[n][x] ? 1.0f : ex2(m[n][x] - m_new);
+                        m[n][x] = m_new;
+                        neg[n][x] = kShift - (m_new == -INFINITY ? 0.0f : m_new);
+                        l[n][x] *= f[x];
+                        f[x] *= fv;
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        o[n][i][0] *= f[0];
+                        o[n][i][1] *= f[1];
+                        o[n][i][2] *= f[0];
+                        o[n][i][3] *= f[1];
+                    }
+                }
+            }
+            uint32_t pb[NT][2], pl[NT][2];  // P^T as the B operand (and its low half)
+            float vf[2] = {1.0f, 1.0f};
+            if constexpr (E4M3) {
+                vf[0] = pow2(static_cast<int>(ex[0] >> 8) - r_v);
+                vf[1] = pow2(static_cast<int>(ex[1] >> 8) - r_v);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    p[n][i] = ex2(p[n][i] + neg[n][i & 1]);
+                    l[n][i & 1] += p[n][i];
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const float lo = p[n][2 * x], hi = p[n][2 * x + 1];
+                    if constexpr (E4M3) {
+                        // A key that is not there has weight 0 and a byte that may be anything.
+                        const float f = tail && g + 8 * x >= limit ? 0.0f : vf[x];
+                        pb[n][x] = transpose8x8(pack2_out(lo * f, hi * f, 1));
+                    } else {
+                        const uint32_t w = pack2_bf16(lo, hi);
+                        pb[n][x] = transpose8x8(w);
+                        pl[n][x] = transpose8x8(pack2_bf16(lo - bf16_lo(w), hi - bf16_hi(w)));
+                    }
+                }
+            }
+            bool odd = false;
+            if (tail) {
+                // Values of keys that are not there are anything, NaN too: as zeros they add nothing.
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const bool here = 2 * t + (x & 1) + 8 * (x >> 1) < limit;
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) {
+                        vr[x][w] = here ? vr[x][w] : 0u;
+                        odd |= odd_word<E4M3>(vr[x][w]);
+                    }
+                }
+            }
+            if (tail && __any_sync(0xffffffffu, odd)) {
+                // An infinity or NaN that some rows see and others do not: token by token, with the keys
+                // that the token does not see as zeros.
+                const int first = r_base / a.group, last = (r_base + n_rows - 1) / a.group;
+                for (int tok = first; tok <= last; ++tok) {
+                    const int lim = there ? s.len - s.rows + tok + 1 - key0 : 0;
+                    uint32_t vm[4][VW];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const bool here = 2 * t + (x & 1) + 8 * (x >> 1) < lim;
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) vm[x][w] = here ? vr[x][w] : 0u;
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        uint32_t f[4];
+                        v_operand<E4M3, VW>(vm, i, f);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma16816<E4M3>(c, f[0], f[1], f[2], f[3], pb[n][0], pb[n][1]);
+                            if constexpr (!E4M3) mma16816<false>(c, f[0], f[1], f[2], f[3], pl[n][0], pl[n][1]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if ((r_base + n * 8 + 2 * t + (j & 1)) / a.group == tok) o[n][i][j] += c[j];
+                            }
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    uint32_t f[4];
+                    v_operand<E4M3, VW>(vr, i, f);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma16816<E4M3>(o[n][i], f[0], f[1], f[2], f[3], pb[n][0], pb[n][1]);
+                        if constexpr (!E4M3) {
+                            mma16816<false>(o[n][i], f[0], f[1], f[2], f[3], pl[n][0], pl[n][1]);
+                        }
+                    }
+                }
+            }
+            if (it + 1 < steps) load_v(next_safe);
+            page = next;
+            ex[0] = ex_next[0];
+            ex[1] = ex_next[1];
+        }
+
+        // Join the warps.
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 4);
+                l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 8);
+                l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 16);
+                if (g == 0) {
+                    m_s[warp][n * 8 + 2 * t + x] = m[n][x];
+                    l_s[warp][n * 8 + 2 * t + x] = l[n][x];
+                }
+            }
+        }
+        __syncthreads();
+        const float f_v = E4M3 ? exp_of_byte(static_cast<uint32_t>(max(r_v, 0))) : 1.0f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int r = n * 8 + 2 * t + x;
+                float top = m_s[0][r];
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][r]);
+                const float f = (m[n][x] == top ? 1.0f : ex2(m[n][x] - top)) * f_v;
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const int v0 = 2 * i;  // the lane's values 2i, 2i + 1 are neighbours
+                    const int d = E4M3 ? g * (D / 8) + v0 : (v0 / 8) * 64 + g * 8 + v0 % 8;
+                    *reinterpret_cast<float2*>(&o_s[warp][r][d]) =
+                        make_float2(o[n][i][x] * f, o[n][i][x + 2] * f);
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = p0 == 0 && p1 == pages;
+        const int part = p0 > 0 ? 0 : 1;
+        for (int at = tid; at < n_rows * (D / 4); at += kThreads) {
+            const int r = at / (D / 4), d = at % (D / 4) * 4;
+            float top = m_s[0][r];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][r]);
+            float sum = 0.0f;
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                sum += l_s[w][r] * (m_s[w][r] == top ? 1.0f : ex2(m_s[w][r] - top));
+                const float4 z = *reinterpret_cast<const float4*>(&o_s[w][r][d]);
+                y.x += z.x;
+                y.y += z.y;
+                y.z += z.z;
+                y.w += z.w;
+            }
+            if (whole && a.prefix_len == 0) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing is zeros
+                const int rr = r_base + r;
+                uint16_t* out = static_cast<uint16_t*>(a.out) + (s.row0 + rr / a.group) * a.out_stride +
+                                (h * a.group + rr % a.group) * D + d;
+                *reinterpret_cast<uint2*>(out) = make_uint2(pack2_out(y.x * inv, y.y * inv, a.f16),
+                                                            pack2_out(y.z * inv, y.w * inv, a.f16));
+            } else if (whole) {
+                const size_t row = h * static_cast<size_t>(a.prefix_rows) +
+                                   static_cast<size_t>(s.row0) * a.group + r_base + r;
+                *reinterpret_cast<float4*>(a.whole_o + row * D + d) = y;
+                if (d == 0) a.whole_ml[row] = make_float2(top, sum);
+            } else {
+                const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + part;
+                *reinterpret_cast<float4*>(a.own_o + (slot * ROWS + r) * D + d) = y;
+                if (d == 0) a.own_ml[slot * ROWS + r] = make_float2(top, sum);
+            }
+        }
+        __syncthreads();
+        pos += p1 - p0;
+    }
+}
+
+// Joins a row's parts: those of its sequence's own pages, where blocks cut them or a prefix adds to
+// them, and the prefix's. One block per (sequence, KV head); a warp takes every fourth row.
+template <int D, int NT>
+__global__ void __launch_bounds__(kThreads) join_kernel(const PagedArgs a) {
+    constexpr int ROWS = 8 * NT, V = D / 32;
+    const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31;
+    const SeqShape s = seq_shape(a, b);
+    const int pages = seq_pages(s), groups = row_groups<NT>(s, a.group);
+    pdl_wait();
+    const long long per = a.first_unit[a.n_seqs + 1];
+    for (int r = threadIdx.x >> 5; r < s.rows * a.group; r += kWarps) {
+        const long long u0 = a.first_unit[b] + (static_cast<long long>(h) * groups + r / ROWS) * pages;
+        const long long c0 = u0 / per, c1 = pages ? (u0 + pages - 1) / per : c0 - 1;
+        if (a.prefix_len == 0 && c0 == c1) continue;  // finished by its block
+        const int token = s.row0 + r / a.group;
+        const int own = static_cast<int>(c1 - c0 + 1), n = own + a.prefix_splits;
+        const size_t row = h * static_cast<size_t>(a.prefix_rows) +
+                           static_cast<size_t>(s.row0) * a.group + r;
+        const size_t split = static_cast<size_t>(a.n_kv) * a.prefix_rows;
+        // Part i: where its (m, l) and its sums lie.
+        auto part_of = [&](int i, const float2*& ml, const float*& o) {
+            if (i >= own) {
+                const size_t at = (i - own) * split + row;
+                ml = a.prefix_ml + at;
+                o = a.prefix_o + at * D;
+            } else if (own == 1) {
+                ml = a.whole_ml + row;
+                o = a.whole_o + row * D;
+            } else {
+                const size_t at = ((c0 + i) * 2 + (i == 0)) * ROWS + r % ROWS;
+                ml = a.own_ml + at;
+                o = a.own_o + at * D;
+            }
+        };
+        const float2* ml;
+        const float* o;
+        float top = -INFINITY;
+        for (int i = lane; i < n; i += 32) {
+            part_of(i, ml, o);
+            top = fmaxf(top, ml->x);
+        }
+        top = warp_max(top);
+        float sum = 0.0f, y[V] = {};
+        for (int i = 0; i < n; ++i) {
+            part_of(i, ml, o);
+            const float f = ml->x == top ? 1.0f : ex2(ml->x - top);
+            sum += ml->y * f;
+#pragma unroll
+            for (int d = 0; d < V; ++d) y[d] = fmaf(o[lane * V + d], f, y[d]);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint16_t* out = static_cast<uint16_t*>(a.out) + token * a.out_stride +
+                        (h * a.group + r % a.group) * D + lane * V;
+#pragma unroll
+        for (int d = 0; d < V; d += 2) {
+            *reinterpret_cast<uint32_t*>(out + d) = pack2_out(y[d] * inv, y[d + 1] * inv, a.f16);
+        }
+    }
+}
+
+template <int D, bool E4M3, int NT>
+void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
+    constexpr int PER_SM = NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2);
+    const long long groups = (static_cast<long long>(a.max_q) * a.group + 8 * NT - 1) / (8 * NT);
+    // No more blocks than the table's width could fill.
+    const long long most = (static_cast<long long>(a.n_seqs) * a.n_kv * a.table_stride * groups +
+                            kMinPages - 1) / kMinPages;
+    const int grid = static_cast<int>(
+        std::max(1LL, std::min({most, static_cast<long long>(sms) * PER_SM, static_cast<long long>(kMaxBlocks)})));
+    launch_dep(false, own_pages_kernel<D, E4M3, NT>, dim3(grid), dim3(kThreads), 0, s, a);
+    launch_dep(true, join_kernel<D, NT>, dim3(a.n_seqs, a.n_kv), dim3(kThreads), 0, s, a);
+}
+
+template <int D, bool E4M3>
+void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
+    if (a.max_q * a.group <= 8) launch_own<D, E4M3, 1>(a, sms, s);
+    else launch_own<D, E4M3, 2>(a, sms, s);
+}
 
 __device__ __forceinline__ float value16(const void* p, size_t i, int f16) {
     const uint16_t u = static_cast<const uint16_t*>(p)[i];
@@ -60,7 +703,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const PagedArgs a) {
 #pragma unroll
             for (int d = 0; d < V; ++d) {
                 const size_t at = row * D + lane * V + d;
-                if (a.e4m3) {
+                if (a.exps) {
                     kx[d] = f16_lo(e4m3x2_to_f16x2(static_cast<const uint8_t*>(a.k)[at])) *
                             exp_of_byte(a.exps[row * 2]);
                     vx[d] = f16_lo(e4m3x2_to_f16x2(static_cast<const uint8_t*>(a.v)[at])) *
@@ -91,12 +734,35 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(const PagedArgs a) {
     }
 }
 
+// ------------------------------------------------------------------ host
+
 constexpr int kMaxGroup = 64, kMaxRows = 128;
 
 bool sizes_ok(const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs, int max_q, int prefix_len) {
     return n_heads > 0 && n_heads % pool->n_kv_heads == 0 && n_heads / pool->n_kv_heads <= kMaxGroup &&
            n_q >= 0 && n_seqs >= 0 && max_q > 0 &&
            static_cast<long long>(max_q) * (n_heads / pool->n_kv_heads) <= kMaxRows && prefix_len >= 0;
+}
+
+// Lays the workspace out from its start; returns its size.
+size_t lay_out(PagedArgs& a, uint8_t* base, int head_dim) {
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t* p = base + at;
+        at += (bytes + 255) & ~size_t(255);
+        return p;
+    };
+    const size_t rows = a.max_q * a.group <= 8 ? 8 : 16;
+    a.first_unit = reinterpret_cast<long long*>(take((static_cast<size_t>(a.n_seqs) + 2) * 8));
+    a.own_ml = reinterpret_cast<float2*>(take(kMaxBlocks * 2 * rows * 8));
+    a.own_o = reinterpret_cast<float*>(take(kMaxBlocks * 2 * rows * head_dim * 4));
+    if (a.prefix_len > 0) {
+        a.prefix_rows = a.n_q * a.group;
+        const size_t all = static_cast<size_t>(a.n_kv) * a.prefix_rows;
+        a.whole_ml = reinterpret_cast<float2*>(take(all * 8));
+        a.whole_o = reinterpret_cast<float*>(take(all * head_dim * 4));
+    }
+    return at;
 }
 
 void paged_attention(void* out, void* workspace, const void* q, int type, int64_t q_stride,
@@ -147,11 +813,19 @@ void paged_attention(void* out, void* workspace, const void* q, int type, int64_
     a.table_stride = table_stride;
     a.prefix_len = prefix_len;
     a.f16 = type == Q3_TYPE_F16;
-    a.e4m3 = pool->type == Q3_TYPE_E4M3;
-    const dim3 grid(n_seqs * max_q, (n_heads + 3) / 4);
+    lay_out(a, static_cast<uint8_t*>(workspace), pool->head_dim);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    launch_dep(false, pool->head_dim == 64 ? attn_rows_kernel<64> : attn_rows_kernel<128>, grid,
-               dim3(128), 0, s, a);
+    const bool e4m3 = pool->type == Q3_TYPE_E4M3;
+    if (prefix_len > 0) {
+        launch_dep(false, pool->head_dim == 64 ? attn_rows_kernel<64> : attn_rows_kernel<128>,
+                   dim3(n_seqs * max_q, (n_heads + 3) / 4), dim3(128), 0, s, a);
+        return;
+    }
+    if (pool->head_dim == 64) {
+        e4m3 ? launch_own<64, true>(a, on.sm_count(), s) : launch_own<64, false>(a, on.sm_count(), s);
+    } else {
+        e4m3 ? launch_own<128, true>(a, on.sm_count(), s) : launch_own<128, false>(a, on.sm_count(), s);
+    }
 }
 
 }  // namespace
@@ -166,7 +840,14 @@ size_t q3_paged_attn_workspace_size(const q3_kv_pool* pool, int n_heads, int n_q
         !q3::sizes_ok(pool, n_heads, n_q, n_seqs, max_q, prefix_len)) {
         return 0;
     }
-    return 256;
+    q3::PagedArgs a{};
+    a.n_kv = pool->n_kv_heads;
+    a.group = n_heads / pool->n_kv_heads;
+    a.n_q = n_q;
+    a.n_seqs = n_seqs;
+    a.max_q = max_q;
+    a.prefix_len = prefix_len;
+    return q3::lay_out(a, nullptr, pool->head_dim);
 }
 
 q3_status q3_paged_attn(void* out, void* workspace, const void* q, int type, int64_t q_stride,

@@ -1,0 +1,85 @@
+// What the kernels of q3_paged_attn / q3_prefix_attn share: arguments, the partition of the work over
+// a sequence's own pages, and the layout of the workspace.
+#pragma once
+
+#include "q3_paged.cuh"
+
+namespace q3 {
+
+struct PagedArgs {
+    void* out;
+    const void* q;
+    const void* k;
+    const void* v;
+    const uint8_t* exps;
+    const int32_t* q_start;
+    const int32_t* kv_len;
+    const int32_t* table;
+    const int32_t* prefix_table;
+    long long q_stride, out_stride;
+    int n_pages, n_kv, group, n_q, n_seqs, max_q, table_stride, prefix_len;
+    int f16;         // q and out are fp16 (else bf16)
+    // Workspace. Partial results are in fp32: o = sum p v and (m, l) = (max of the scores in units of
+    // log2, sum p), p = 2^(score - m + kShift).
+    long long* first_unit;  // [n_seqs + 2]: units before each sequence, all of them, units a block
+    float* own_o;           // [blocks][2][8 * tiles][head_dim]
+    float2* own_ml;         // [blocks][2][8 * tiles]
+    float* whole_o;         // [n_kv][prefix_rows][head_dim]: with a prefix, own parts that were not cut
+    float2* whole_ml;       // [n_kv][prefix_rows]
+    float* prefix_o;        // [splits][n_kv][prefix_rows][head_dim]
+    float2* prefix_ml;      // [splits][n_kv][prefix_rows]
+    int prefix_splits, prefix_rows;
+};
+
+constexpr float kShift = 8.0f;     // the weights' largest is about 2^8: fp16 then reaches to 2^-32 of it
+constexpr int kMaxBlocks = 640;    // of the own-pages kernel: at least 4 a multiprocessor
+constexpr int kMinPages = 8;       // a block's smallest share of pages
+
+// Rows of sequence b and its own tokens, whatever the arrays hold.
+struct SeqShape {
+    int row0, rows, len;
+};
+__device__ __forceinline__ SeqShape seq_shape(const PagedArgs& a, int b) {
+    SeqShape s;
+    s.row0 = min(max(a.q_start[b], 0), a.n_q);
+    s.rows = min(min(a.q_start[b + 1], a.n_q) - s.row0, a.max_q);
+    s.rows = max(s.rows, 0);
+    s.len = static_cast<int>(min(static_cast<long long>(max(a.kv_len[b], 0)),
+                                 static_cast<long long>(a.table_stride) * kPageTokens));
+    return s;
+}
+
+// Row r of (sequence, KV head): query token r / group, query head r % group of the KV head's.
+__device__ __forceinline__ int seq_pages(const SeqShape& s) {
+    return static_cast<int>((static_cast<long long>(s.len) + kPageTokens - 1) / kPageTokens);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 2^e for any int e (0 below the normal range, infinity above).
+__device__ __forceinline__ float pow2(int e) {
+    return e < -126 ? 0.0f : e > 127 ? INFINITY : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+__device__ __forceinline__ uint32_t pack2_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// Two results in the caller's type, to nearest even; an fp16 result past the range becomes infinity.
+__device__ __forceinline__ uint32_t pack2_out(float lo, float hi, int f16) {
+    if (!f16) return pack2_bf16(lo, hi);
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+void launch_prefix_attention(const PagedArgs& a, int head_dim, bool e4m3, int sms, cudaStream_t s);
+// KV splits of the prefix kernel, from the sizes alone.
+int prefix_splits(int n_kv, int rows, int prefix_len);
+
+}  // namespace q3
