@@ -177,7 +177,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3
             a.first_unit[a.n_seqs + 1] = per;
         }
     }
-    if (start >= end) return;
+    if (start >= end) {
+        pdl_wait();
+        return;
+    }
     if (before <= start && start < before + mine) {
         long long x = before;
         int b = b0;
@@ -584,6 +587,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3
         __syncthreads();
         pos += p1 - p0;
     }
+    // This grid may have started beside the prefix's, which it does not read; join_kernel waits for this
+    // one alone, so this one ends after that.
+    pdl_wait();
 }
 
 // Joins a row's parts: those of its sequence's own pages, where blocks cut them or a prefix adds to
@@ -655,7 +661,7 @@ void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
                             kMinPages - 1) / kMinPages;
     const int grid = static_cast<int>(
         std::max(1LL, std::min({most, static_cast<long long>(sms) * PER_SM, static_cast<long long>(kMaxBlocks)})));
-    launch_dep(false, own_pages_kernel<D, E4M3, NT>, dim3(grid), dim3(kThreads), 0, s, a);
+    launch_dep(a.prefix_len > 0, own_pages_kernel<D, E4M3, NT>, dim3(grid), dim3(kThreads), 0, s, a);
     launch_dep(true, join_kernel<D, NT>, dim3(a.n_seqs, a.n_kv), dim3(kThreads), 0, s, a);
 }
 
@@ -665,83 +671,15 @@ void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
     else launch_own<D, E4M3, 2>(a, sms, s);
 }
 
-__device__ __forceinline__ float value16(const void* p, size_t i, int f16) {
-    const uint16_t u = static_cast<const uint16_t*>(p)[i];
-    return f16 ? __half2float(__ushort_as_half(u)) : bf16_to_f32(u);
-}
-
-// One warp per (row, query head), a lane per D / 32 values of the head.
-template <int D>
-__global__ void __launch_bounds__(128) attn_rows_kernel(const PagedArgs a) {
-    constexpr int V = D / 32;
-    const int lane = threadIdx.x & 31, heads = a.n_kv * a.group;
-    const int head = blockIdx.y * 4 + (threadIdx.x >> 5);
-    const int b = blockIdx.x / a.max_q, i = blockIdx.x % a.max_q;
-    if (head >= heads) return;
-    const int r0 = max(a.q_start[b], 0), r1 = min(a.q_start[b + 1], a.n_q);
-    const int rows = min(r1 - r0, a.max_q);
-    if (i >= rows) return;
-    const int kvh = head / a.group;
-    const int len = static_cast<int>(
-        min(static_cast<long long>(max(a.kv_len[b], 0)), static_cast<long long>(a.table_stride) * kPageTokens));
-    const int seen = max(0, len - rows + i + 1);
-    float q[V], o[V] = {};
-#pragma unroll
-    for (int d = 0; d < V; ++d) {
-        q[d] = value16(a.q, (r0 + i) * a.q_stride + head * D + lane * V + d, a.f16) *
-               (1.4426950408889634f / sqrtf(static_cast<float>(D)));
-    }
-    float m = -INFINITY, l = 0.0f;
-    for (int part = 0; part < 2; ++part) {
-        const int32_t* table = part ? a.table + static_cast<size_t>(b) * a.table_stride : a.prefix_table;
-        const int keys = part ? seen : a.prefix_len;
-        for (int j = 0; j < keys; ++j) {
-            const int page = table[j / kPageTokens];
-            if (page < 0 || page >= a.n_pages) continue;
-            const size_t row = (static_cast<size_t>(page) * a.n_kv + kvh) * kPageTokens + j % kPageTokens;
-            float kx[V], vx[V];
-#pragma unroll
-            for (int d = 0; d < V; ++d) {
-                const size_t at = row * D + lane * V + d;
-                if (a.exps) {
-                    kx[d] = f16_lo(e4m3x2_to_f16x2(static_cast<const uint8_t*>(a.k)[at])) *
-                            exp_of_byte(a.exps[row * 2]);
-                    vx[d] = f16_lo(e4m3x2_to_f16x2(static_cast<const uint8_t*>(a.v)[at])) *
-                            exp_of_byte(a.exps[row * 2 + 1]);
-                } else {
-                    kx[d] = bf16_to_f32(static_cast<const uint16_t*>(a.k)[at]);
-                    vx[d] = bf16_to_f32(static_cast<const uint16_t*>(a.v)[at]);
-                }
-            }
-            float s = 0.0f;
-#pragma unroll
-            for (int d = 0; d < V; ++d) s = fmaf(q[d], kx[d], s);
-            s = warp_sum(s);
-            const float m_new = fmaxf(m, s);
-            const float f = m_new == -INFINITY ? 1.0f : exp2f(m - m_new);
-            const float p = m_new == -INFINITY ? 0.0f : exp2f(s - m_new);
-            l = l * f + p;
-#pragma unroll
-            for (int d = 0; d < V; ++d) o[d] = fmaf(p, vx[d], o[d] * f);
-            m = m_new;
-        }
-    }
-#pragma unroll
-    for (int d = 0; d < V; ++d) {
-        const float y = l == 0.0f ? 0.0f : o[d] / l;  // a row that sees nothing is zeros
-        static_cast<uint16_t*>(a.out)[(r0 + i) * a.out_stride + head * D + lane * V + d] =
-            a.f16 ? __half_as_ushort(__float2half_rn(y)) : f32_to_bf16(y);
-    }
-}
-
 // ------------------------------------------------------------------ host
 
-constexpr int kMaxGroup = 64, kMaxRows = 128;
+constexpr int kMaxGroup = 64, kMaxRows = 128, kMaxBatchRows = 1 << 23;
 
 bool sizes_ok(const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs, int max_q, int prefix_len) {
     return n_heads > 0 && n_heads % pool->n_kv_heads == 0 && n_heads / pool->n_kv_heads <= kMaxGroup &&
            n_q >= 0 && n_seqs >= 0 && max_q > 0 &&
-           static_cast<long long>(max_q) * (n_heads / pool->n_kv_heads) <= kMaxRows && prefix_len >= 0;
+           static_cast<long long>(max_q) * (n_heads / pool->n_kv_heads) <= kMaxRows && prefix_len >= 0 &&
+           static_cast<long long>(n_q) * (n_heads / pool->n_kv_heads) <= kMaxBatchRows;
 }
 
 // Lays the workspace out from its start; returns its size.
@@ -761,6 +699,9 @@ size_t lay_out(PagedArgs& a, uint8_t* base, int head_dim) {
         const size_t all = static_cast<size_t>(a.n_kv) * a.prefix_rows;
         a.whole_ml = reinterpret_cast<float2*>(take(all * 8));
         a.whole_o = reinterpret_cast<float*>(take(all * head_dim * 4));
+        a.prefix_splits = prefix_splits(a.n_kv, a.prefix_rows, a.prefix_len);
+        a.prefix_ml = reinterpret_cast<float2*>(take(a.prefix_splits * all * 8));
+        a.prefix_o = reinterpret_cast<float*>(take(a.prefix_splits * all * head_dim * 4));
     }
     return at;
 }
@@ -816,11 +757,7 @@ void paged_attention(void* out, void* workspace, const void* q, int type, int64_
     lay_out(a, static_cast<uint8_t*>(workspace), pool->head_dim);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool e4m3 = pool->type == Q3_TYPE_E4M3;
-    if (prefix_len > 0) {
-        launch_dep(false, pool->head_dim == 64 ? attn_rows_kernel<64> : attn_rows_kernel<128>,
-                   dim3(n_seqs * max_q, (n_heads + 3) / 4), dim3(128), 0, s, a);
-        return;
-    }
+    if (prefix_len > 0) launch_prefix_attention(a, pool->head_dim, e4m3, s);
     if (pool->head_dim == 64) {
         e4m3 ? launch_own<64, true>(a, on.sm_count(), s) : launch_own<64, false>(a, on.sm_count(), s);
     } else {

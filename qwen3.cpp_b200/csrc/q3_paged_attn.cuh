@@ -78,8 +78,8 @@ __device__ __forceinline__ uint32_t pack2_out(float lo, float hi, int f16) {
     return r;
 }
 
-void launch_prefix_attention(const PagedArgs& a, int head_dim, bool e4m3, int sms, cudaStream_t s);
-// KV splits of the prefix kernel, from the sizes alone.
+void launch_prefix_attention(const PagedArgs& a, int head_dim, bool e4m3, cudaStream_t s);
+// Parts that the prefix kernel leaves for each row, from the sizes alone.
 int prefix_splits(int n_kv, int rows, int prefix_len);
 
 }  // namespace q3
