@@ -3,10 +3,11 @@
 //
 // own_pages_kernel computes the part over each sequence's own pages, join_kernel joins the parts.
 //
-// Work: a unit is one page of one (sequence, KV head, group of 8 * NT rows). The units of all
+// Work: a strip is the pages of one (sequence, KV head, group of 8 * NT rows); its units are its pages
+// and kSetup more in front, for what a strip costs before and after its pages. The units of all
 // sequences form one line, cut into equal runs, one a block, so a ragged batch loads every block
 // alike and a long sequence spreads over many. Each block finds its run from the lengths on the
-// device (a scan over the sequences), so a captured graph follows them. A (sequence, head, group)
+// device (a scan over the sequences), so a captured graph follows them. A strip whose pages lie
 // inside one run is finished there; one that is cut leaves a part per block, at most two a block, and
 // join_kernel adds them by their softmax statistics.
 //
@@ -14,10 +15,14 @@
 //   S^T[16 keys x 8 rows] = K . Q^T      K's rows are the A operand as they lie in memory
 //   O^T[d x 8 rows]      += V^T . P^T    two keys' V values of one d are a register of A
 // The order of the head's dimensions inside an operand is free as long as both sides agree, so a lane
-// loads 16 contiguous bytes and they are its operand registers (bf16) or become them by a conversion
-// (e4m3 -> fp16, exact); V pairs need one byte permutation. Nothing goes through shared memory: K of
-// page i + 4 is on its way while the scores of page i turn into weights, V while its K is multiplied.
-// The scores come out transposed for the second product; movmatrix turns the rounded weights.
+// takes 16 contiguous bytes and they are its operand registers (bf16) or become them by a conversion
+// (e4m3 -> fp16, exact); V pairs need one byte permutation. The scores come out transposed for the
+// second product; movmatrix turns the rounded weights.
+//
+// Each warp has its own ring of kStages pages in shared memory, filled by cp.async a page or two ahead
+// (registers hold one page at most, and the multiprocessor's 16 warps then have too few bytes on the
+// way: 78 us against 67 for 64 sequences of 128 to 4096 tokens). 16-byte piece c of row r lies at
+// piece c ^ (r % 8), which leaves the operand reads without bank conflicts.
 //
 // The running maximum moves only when a score passes it by more than 2^4 (one vote a page instead of
 // two times three shuffles): weights are then at most 2^(kShift + 4), which fp16 holds, as it does 2^3
@@ -41,6 +46,37 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kGrow = 4.0f;  // how far (log2) a score may pass the running maximum
 constexpr int kGrowV = 3;      // the same for V's powers of two
+
+// Pages of a warp's ring, and blocks a multiprocessor (registers and rings together).
+template <bool E4M3, int NT>
+struct Shape {
+    static constexpr int kStages = E4M3 ? 3 : 2;
+    static constexpr int kBlocks = NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2);
+};
+
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_4(uint32_t to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void lds_16(uint32_t from, uint32_t* r) {
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(from) : "memory");
+}
+__device__ __forceinline__ void lds_8(uint32_t from, uint32_t* r) {
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(from) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t from) {
+    uint16_t r;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(from) : "memory");
+    return r;
+}
 
 template <bool F16>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -66,28 +102,18 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
-template <int BYTES>
-__device__ __forceinline__ void load_bytes(const uint8_t* p, uint32_t* r) {
-    static_assert(BYTES == 8 || BYTES % 16 == 0, "run width");
-    if constexpr (BYTES == 8) {
-        asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
-    } else {
-#pragma unroll
-        for (int i = 0; i < BYTES / 16; ++i) {
-            const uint4 x = ldg_stream(p + 16 * i);
-            r[4 * i] = x.x;
-            r[4 * i + 1] = x.y;
-            r[4 * i + 2] = x.z;
-            r[4 * i + 3] = x.w;
-        }
-    }
-}
-
 // Whether a packed word of pool values holds an infinity or NaN.
 template <bool E4M3>
 __device__ __forceinline__ bool odd_word(uint32_t x) {
     return E4M3 ? (((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0
                 : (((x & 0x7fff7fffu) + 0x00800080u) & 0x80008000u) != 0;
+}
+
+// Piece j (of PIECES / 4) that lane t of its row's four takes of a K row, and of a Q row: neighbours, so
+// that two rows' reads fall into different banks.
+template <int PIECES>
+__device__ __forceinline__ int k_piece(int t, int j) {
+    return PIECES == 4 ? t : (j >> 1) * 8 + 2 * t + (j & 1);
 }
 
 // The A operand of O^T += V^T P^T for m-tile i: a0, a1 from the keys 2t, 2t + 1, a2, a3 from 2t + 8,
@@ -137,14 +163,25 @@ __device__ __forceinline__ int row_groups(const SeqShape& s, int group) {
 }
 
 template <int D, bool E4M3, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2))
+struct OwnSmem {
+    static constexpr int kRow = E4M3 ? D : 2 * D;                  // bytes of a pool row
+    static constexpr int kPage = 2 * kPageTokens * kRow + (E4M3 ? 2 * kPageTokens : 0);  // K, V, bytes
+    static constexpr int kRing = kWarps * Shape<E4M3, NT>::kStages * kPage;
+    static constexpr int kSums = kWarps * 8 * NT * D * 4;          // after a run of pages, in its place
+    static constexpr int kBytes = kRing > kSums ? kRing : kSums;
+};
+
+template <int D, bool E4M3, int NT>
+__global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
     own_pages_kernel(const PagedArgs a) {
     constexpr int MT = D / 16;                    // m-tiles of O^T, k-steps of S^T
     constexpr int KW = E4M3 ? D / 16 : D / 8;     // words a lane holds of one K row
     constexpr int VW = E4M3 ? D / 32 : D / 16;    // and of one V row
-    constexpr int ROW = E4M3 ? D : 2 * D;         // bytes of a pool row
+    using L = OwnSmem<D, E4M3, NT>;
+    constexpr int ROW = L::kRow, PIECES = ROW / 16, STAGES = Shape<E4M3, NT>::kStages;
     constexpr int ROWS = 8 * NT;
-    __shared__ float o_s[kWarps][ROWS][D];
+    extern __shared__ __align__(128) uint8_t ring_s[];
+    float (*o_s)[ROWS][D] = reinterpret_cast<float (*)[ROWS][D]>(ring_s);
     __shared__ float m_s[kWarps][ROWS], l_s[kWarps][ROWS];
     __shared__ long long scan_s[kWarps];
     __shared__ long long first_s;
@@ -158,12 +195,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3
     const int b0 = min(tid * per_thread, a.n_seqs), b1 = min(b0 + per_thread, a.n_seqs);
     auto units = [&](int b) {
         const SeqShape s = seq_shape(a, b);
-        return static_cast<long long>(a.n_kv) * row_groups<NT>(s, a.group) * seq_pages(s);
+        const int pages = seq_pages(s);
+        return pages ? static_cast<long long>(a.n_kv) * row_groups<NT>(s, a.group) * (pages + kSetup) : 0;
     };
     long long mine = 0, before, total;
     for (int b = b0; b < b1; ++b) mine += units(b);
     block_scan(mine, scan_s, before, total);
-    const long long per = max(static_cast<long long>(kMinPages),
+    const long long per = max(static_cast<long long>(kMinUnits),
                               (total + gridDim.x - 1) / static_cast<long long>(gridDim.x));
     const long long start = per * blockIdx.x, end = min(total, start + per);
     if (blockIdx.x == 0) {
@@ -190,26 +228,63 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3
     }
     __syncthreads();
 
-    const uint8_t* kp = static_cast<const uint8_t*>(a.k);
-    const uint8_t* vp = static_cast<const uint8_t*>(a.v);
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(ring_s)) + warp * STAGES * L::kPage;
     const float scale = 1.4426950408889634f / sqrtf(static_cast<float>(D));
     long long pos = start, seq_first = first_s;
     int b = seq_s;
     while (pos < end) {
         const SeqShape s = seq_shape(a, b);
         const int pages = seq_pages(s), groups = row_groups<NT>(s, a.group);
-        const long long all = static_cast<long long>(a.n_kv) * groups * pages;
+        const long long all = pages ? static_cast<long long>(a.n_kv) * groups * (pages + kSetup) : 0;
         if (pos >= seq_first + all) {
             seq_first += all;
             ++b;
             continue;
         }
-        const long long strip = (pos - seq_first) / pages;  // (head, row group)
-        const int p0 = static_cast<int>(pos - seq_first - strip * pages);
-        const int p1 = static_cast<int>(min(static_cast<long long>(pages), p0 + (end - pos)));
+        const long long strip = (pos - seq_first) / (pages + kSetup);  // (head, row group)
+        const long long u0 = pos - seq_first - strip * (pages + kSetup);
+        const long long u1 = min(static_cast<long long>(pages) + kSetup, u0 + (end - pos));
+        const int p0 = static_cast<int>(max(0LL, u0 - kSetup)), p1 = static_cast<int>(u1 - kSetup);
+        pos += u1 - u0;
+        if (p1 <= 0) continue;  // the run ends before the strip's first page
         const int h = static_cast<int>(strip / groups), rg = static_cast<int>(strip % groups);
         const int r_base = rg * ROWS;
         const int n_rows = min(ROWS, s.rows * a.group - r_base);
+
+        // This warp's pages, the first of them on their way.
+        const int32_t* table = a.table + static_cast<size_t>(b) * a.table_stride;
+        const int steps = p1 - p0 > warp ? (p1 - p0 - warp + kWarps - 1) / kWarps : 0;
+        int ids = 0;
+        unsigned good = 0;  // of the last 32 steps looked up: whether the page is in the pool
+        auto start_page = [&](int it) {  // in order: 0, 1, 2, ...
+            if ((it & 31) == 0) {
+                const int p = p0 + warp + (it + lane) * kWarps;
+                ids = p < p1 ? table[p] : -1;
+            }
+            const int page = __shfl_sync(0xffffffffu, ids, it & 31);
+            const bool in = page >= 0 && page < a.n_pages;
+            good = good << 1 | in;
+            // A page that is not there is page 0 in its place, whose keys are masked.
+            const size_t row = (static_cast<size_t>(in ? page : 0) * a.n_kv + h) * kPageTokens;
+            const uint32_t to = ring + (it % STAGES) * L::kPage;
+            const uint8_t* kp = static_cast<const uint8_t*>(a.k) + row * ROW;
+            const uint8_t* vp = static_cast<const uint8_t*>(a.v) + row * ROW;
+#pragma unroll
+            for (int i = 0; i < kPageTokens * PIECES / 32; ++i) {
+                const int x = i * 32 + lane, r = x / PIECES, c = x % PIECES;
+                const uint32_t at = r * ROW + ((c ^ (r & (PIECES < 8 ? PIECES - 1 : 7))) * 16);
+                copy_16(to + at, kp + x * 16);
+                copy_16(to + kPageTokens * ROW + at, vp + x * 16);
+            }
+            if (E4M3 && lane < 8) {
+                copy_4(to + 2 * kPageTokens * ROW + lane * 4, a.exps + row * 2 + lane * 4);
+            }
+        };
+#pragma unroll
+        for (int it = 0; it < STAGES - 1; ++it) {
+            if (it < steps) start_page(it);
+            copy_commit();
+        }
 
         // Q as the B operand: lane (g, t) holds row g's values in the order of K's.
         uint32_t qw[NT][D / 8];
@@ -221,13 +296,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3
             const bool live = n * 8 + g < n_rows;
             const uint16_t* qp = static_cast<const uint16_t*>(a.q) +
                                  (live ? (s.row0 + r / a.group) * a.q_stride + (h * a.group + r % a.group) * D : 0);
-            constexpr int CH = E4M3 ? 16 : 8;  // consecutive values
+            constexpr int CH = E4M3 ? 16 : 8;  // values of a 16-byte piece
 #pragma unroll
-            for (int j = 0; j < D / (4 * CH); ++j) {
+            for (int j = 0; j < PIECES / 4; ++j) {
 #pragma unroll
                 for (int i = 0; i < CH / 8; ++i) {
                     uint4 x = make_uint4(0, 0, 0, 0);
-                    if (live) x = *reinterpret_cast<const uint4*>(qp + j * 4 * CH + t * CH + 8 * i);
+                    if (live) x = *reinterpret_cast<const uint4*>(qp + k_piece<PIECES>(t, j) * CH + 8 * i);
                     uint32_t* w = &qw[n][(j * (CH / 8) + i) * 4];
                     w[0] = x.x;
                     w[1] = x.y;
@@ -282,60 +357,28 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3
             for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
         }
 
-        const int32_t* table = a.table + static_cast<size_t>(b) * a.table_stride;
-        const int steps = p1 - p0 > warp ? (p1 - p0 - warp + kWarps - 1) / kWarps : 0;
-        int ids = 0;
-        auto page_of = [&](int it) {  // page of this warp's step `it` (in order: 0, 1, 2, ...)
-            if ((it & 31) == 0) {
-                const int p = p0 + warp + (it + lane) * kWarps;
-                ids = p < p1 ? table[p] : -1;
-            }
-            return __shfl_sync(0xffffffffu, ids, it & 31);
-        };
-        uint32_t kr[2][KW], vr[4][VW];
-        uint32_t ex[2] = {0, 0};
-        auto load_k = [&](int page) {
-            const size_t row = (static_cast<size_t>(page) * a.n_kv + h) * kPageTokens;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const uint8_t* p = kp + (row + g + 8 * x) * ROW + t * 16;
-#pragma unroll
-                for (int j = 0; j < KW / 4; ++j) load_bytes<16>(p + j * 64, &kr[x][4 * j]);
-            }
-        };
-        auto load_v = [&](int page) {
-            const size_t row = (static_cast<size_t>(page) * a.n_kv + h) * kPageTokens;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const uint8_t* p = vp + (row + 2 * t + (x & 1) + 8 * (x >> 1)) * ROW;
-                if constexpr (E4M3) {
-                    load_bytes<VW * 4>(p + g * (VW * 4), vr[x]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VW / 4; ++j) load_bytes<16>(p + j * 128 + g * 16, &vr[x][4 * j]);
-                }
-            }
-        };
-        auto load_exps = [&](int page, uint32_t (&to)[2]) {
-            if constexpr (E4M3) {
-                const uint16_t* p = reinterpret_cast<const uint16_t*>(a.exps) +
-                                    (static_cast<size_t>(page) * a.n_kv + h) * kPageTokens + g;
-                to[0] = __ldg(p);
-                to[1] = __ldg(p + 8);
-            }
-        };
-
-        int page = -1;
-        if (steps > 0) {
-            page = page_of(0);
-            const int safe = page >= 0 && page < a.n_pages ? page : 0;
-            load_k(safe);
-            load_exps(safe, ex);
-            load_v(safe);
-        }
         for (int it = 0; it < steps; ++it) {
             const int key0 = (p0 + warp + it * kWarps) * kPageTokens;
-            const bool there = page >= 0 && page < a.n_pages;
+            copy_wait<STAGES - 2>();
+            __syncwarp();  // every lane's copies of this page are in, and its reads of the one before done
+            // `good` grows a bit a page looked up: this page's is (pages looked up since) from its end.
+            const bool there = good >> (min(it + STAGES - 2, steps - 1) - it) & 1;
+            if (it + STAGES - 1 < steps) start_page(it + STAGES - 1);
+            copy_commit();
+            const uint32_t page_s = ring + (it % STAGES) * L::kPage;
+            constexpr int SW = PIECES < 8 ? PIECES - 1 : 7;
+            uint32_t kr[2][KW], vr[4][VW], ex[2] = {0, 0};
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int j = 0; j < PIECES / 4; ++j) {
+                    lds_16(page_s + (g + 8 * x) * ROW + ((k_piece<PIECES>(t, j) ^ (g & SW)) * 16), &kr[x][4 * j]);
+                }
+            }
+            if constexpr (E4M3) {
+                ex[0] = lds_u16(page_s + 2 * kPageTokens * ROW + g * 2);
+                ex[1] = lds_u16(page_s + 2 * kPageTokens * ROW + g * 2 + 16);
+            }
             // Scores: two chains of products, so that one is not a wait for the other.
             float sc[NT][2][4];
 #pragma unroll
@@ -361,14 +404,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3
                 for (int n = 0; n < NT; ++n) {
                     mma16816<E4M3>(sc[n][k & 1], f[0], f[1], f[2], f[3], qw[n][2 * k], qw[n][2 * k + 1]);
                 }
-            }
-            int next = -1, next_safe = 0;
-            uint32_t ex_next[2] = {0, 0};
-            if (it + 1 < steps) {
-                next = page_of(it + 1);
-                next_safe = next >= 0 && next < a.n_pages ? next : 0;
-                load_k(next_safe);
-                load_exps(next_safe, ex_next);
             }
             const bool tail = !there || key0 + kPageTokens > tail_key;
             const int limit = there ? s.len - key0 : 0;  // this page's keys that exist
@@ -451,6 +486,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3
                     }
                 }
             }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int r = 2 * t + (x & 1) + 8 * (x >> 1);
+                const uint32_t at = page_s + (kPageTokens + r) * ROW;
+                if constexpr (E4M3 && D == 64) {
+                    lds_8(at + (((g >> 1) ^ (r & SW)) * 16) + (g & 1) * 8, vr[x]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VW / 4; ++j) lds_16(at + (((j * 8 + g) ^ (r & SW)) * 16), &vr[x][4 * j]);
+                }
+            }
             bool odd = false;
             if (tail) {
                 // Values of keys that are not there are anything, NaN too: as zeros they add nothing.
@@ -507,10 +553,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3
                     }
                 }
             }
-            if (it + 1 < steps) load_v(next_safe);
-            page = next;
-            ex[0] = ex_next[0];
-            ex[1] = ex_next[1];
         }
 
         // Join the warps.
@@ -585,7 +627,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3
             }
         }
         __syncthreads();
-        pos += p1 - p0;
     }
     // This grid may have started beside the prefix's, which it does not read; join_kernel waits for this
     // one alone, so this one ends after that.
@@ -593,76 +634,95 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3
 }
 
 // Joins a row's parts: those of its sequence's own pages, where blocks cut them or a prefix adds to
-// them, and the prefix's. One block per (sequence, KV head); a warp takes every fourth row.
+// them, and the prefix's. A warp a row: a lane looks up a part's weight and place, then all lanes add
+// the part's sums, several parts on their way at once.
 template <int D, int NT>
 __global__ void __launch_bounds__(kThreads) join_kernel(const PagedArgs a) {
     constexpr int ROWS = 8 * NT, V = D / 32;
-    const int b = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31;
-    const SeqShape s = seq_shape(a, b);
+    const int lane = threadIdx.x & 31, most = a.max_q * a.group;
+    const long long w = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    const int r = static_cast<int>(w % most), h = static_cast<int>(w / most % a.n_kv);
+    const long long b = w / most / a.n_kv;
+    if (b >= a.n_seqs) return;
+    const SeqShape s = seq_shape(a, static_cast<int>(b));
+    if (r >= s.rows * a.group) return;
     const int pages = seq_pages(s), groups = row_groups<NT>(s, a.group);
     pdl_wait();
     const long long per = a.first_unit[a.n_seqs + 1];
-    for (int r = threadIdx.x >> 5; r < s.rows * a.group; r += kWarps) {
-        const long long u0 = a.first_unit[b] + (static_cast<long long>(h) * groups + r / ROWS) * pages;
-        const long long c0 = u0 / per, c1 = pages ? (u0 + pages - 1) / per : c0 - 1;
-        if (a.prefix_len == 0 && c0 == c1) continue;  // finished by its block
-        const int token = s.row0 + r / a.group;
-        const int own = static_cast<int>(c1 - c0 + 1), n = own + a.prefix_splits;
-        const size_t row = h * static_cast<size_t>(a.prefix_rows) +
-                           static_cast<size_t>(s.row0) * a.group + r;
-        const size_t split = static_cast<size_t>(a.n_kv) * a.prefix_rows;
-        // Part i: where its (m, l) and its sums lie.
-        auto part_of = [&](int i, const float2*& ml, const float*& o) {
+    const long long u0 = a.first_unit[b] + kSetup +
+                         (static_cast<long long>(h) * groups + r / ROWS) * (pages + kSetup);
+    const long long c0 = u0 / per, c1 = pages ? (u0 + pages - 1) / per : c0 - 1;
+    if (a.prefix_len == 0 && c0 == c1) return;  // finished by its block
+    const int own = static_cast<int>(c1 - c0 + 1), n = own + a.prefix_splits;
+    const size_t row = h * static_cast<size_t>(a.prefix_rows) + static_cast<size_t>(s.row0) * a.group + r;
+    const size_t split = static_cast<size_t>(a.n_kv) * a.prefix_rows;
+    float top = -INFINITY, sum = 0.0f;  // sum: this lane's parts
+    float y[V] = {};
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int i = i0 + lane;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        const float* o = nullptr;
+        if (i < n) {
+            const float2* p;
             if (i >= own) {
                 const size_t at = (i - own) * split + row;
-                ml = a.prefix_ml + at;
+                p = a.prefix_ml + at;
                 o = a.prefix_o + at * D;
             } else if (own == 1) {
-                ml = a.whole_ml + row;
+                p = a.whole_ml + row;
                 o = a.whole_o + row * D;
             } else {
                 const size_t at = ((c0 + i) * 2 + (i == 0)) * ROWS + r % ROWS;
-                ml = a.own_ml + at;
+                p = a.own_ml + at;
                 o = a.own_o + at * D;
             }
-        };
-        const float2* ml;
-        const float* o;
-        float top = -INFINITY;
-        for (int i = lane; i < n; i += 32) {
-            part_of(i, ml, o);
-            top = fmaxf(top, ml->x);
+            ml = *p;
         }
-        top = warp_max(top);
-        float sum = 0.0f, y[V] = {};
-        for (int i = 0; i < n; ++i) {
-            part_of(i, ml, o);
-            const float f = ml->x == top ? 1.0f : ex2(ml->x - top);
-            sum += ml->y * f;
+        const float top_new = fmaxf(top, warp_max(ml.x));
+        const float back = top_new == top ? 1.0f : ex2(top - top_new);
+        const float f = ml.x == top_new ? 1.0f : ex2(ml.x - top_new);
+        top = top_new;
+        sum = fmaf(ml.y, f, sum * back);
 #pragma unroll
-            for (int d = 0; d < V; ++d) y[d] = fmaf(o[lane * V + d], f, y[d]);
-        }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        uint16_t* out = static_cast<uint16_t*>(a.out) + token * a.out_stride +
-                        (h * a.group + r % a.group) * D + lane * V;
+        for (int d = 0; d < V; ++d) y[d] *= back;
+        const int here = min(32, n - i0);
+#pragma unroll 8
+        for (int x = 0; x < here; ++x) {
+            const float* ox = reinterpret_cast<const float*>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), x));
+            const float fx = __shfl_sync(0xffffffffu, f, x);
+            float z[V];
+            if constexpr (V == 4) *reinterpret_cast<float4*>(z) = *reinterpret_cast<const float4*>(ox + lane * V);
+            else *reinterpret_cast<float2*>(z) = *reinterpret_cast<const float2*>(ox + lane * V);
 #pragma unroll
-        for (int d = 0; d < V; d += 2) {
-            *reinterpret_cast<uint32_t*>(out + d) = pack2_out(y[d] * inv, y[d + 1] * inv, a.f16);
+            for (int d = 0; d < V; ++d) y[d] = fmaf(z[d], fx, y[d]);
         }
     }
+    sum = warp_sum(sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + (s.row0 + r / a.group) * a.out_stride +
+                    (h * a.group + r % a.group) * D + lane * V;
+    uint32_t z[V / 2];
+#pragma unroll
+    for (int d = 0; d < V; d += 2) z[d / 2] = pack2_out(y[d] * inv, y[d + 1] * inv, a.f16);
+    if constexpr (V == 4) *reinterpret_cast<uint2*>(out) = make_uint2(z[0], z[1]);
+    else *reinterpret_cast<uint32_t*>(out) = z[0];
 }
 
 template <int D, bool E4M3, int NT>
 void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
-    constexpr int PER_SM = NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2);
     const long long groups = (static_cast<long long>(a.max_q) * a.group + 8 * NT - 1) / (8 * NT);
     // No more blocks than the table's width could fill.
-    const long long most = (static_cast<long long>(a.n_seqs) * a.n_kv * a.table_stride * groups +
-                            kMinPages - 1) / kMinPages;
-    const int grid = static_cast<int>(
-        std::max(1LL, std::min({most, static_cast<long long>(sms) * PER_SM, static_cast<long long>(kMaxBlocks)})));
-    launch_dep(a.prefix_len > 0, own_pages_kernel<D, E4M3, NT>, dim3(grid), dim3(kThreads), 0, s, a);
-    launch_dep(true, join_kernel<D, NT>, dim3(a.n_seqs, a.n_kv), dim3(kThreads), 0, s, a);
+    const long long most = (static_cast<long long>(a.n_seqs) * a.n_kv * (a.table_stride + kSetup) * groups +
+                            kMinUnits - 1) / kMinUnits;
+    const int grid = static_cast<int>(std::max(
+        1LL, std::min({most, static_cast<long long>(sms) * Shape<E4M3, NT>::kBlocks, static_cast<long long>(kMaxBlocks)})));
+    constexpr int bytes = OwnSmem<D, E4M3, NT>::kBytes;
+    Q3_CUDA(cudaFuncSetAttribute(own_pages_kernel<D, E4M3, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    launch_dep(a.prefix_len > 0, own_pages_kernel<D, E4M3, NT>, dim3(grid), dim3(kThreads), bytes, s, a);
+    const long long rows = static_cast<long long>(a.n_seqs) * a.n_kv * a.max_q * a.group;
+    launch_dep(true, join_kernel<D, NT>, dim3(static_cast<unsigned>((rows + kWarps - 1) / kWarps)),
+               dim3(kThreads), 0, s, a);
 }
 
 template <int D, bool E4M3>
@@ -679,7 +739,8 @@ bool sizes_ok(const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs, int max_
     return n_heads > 0 && n_heads % pool->n_kv_heads == 0 && n_heads / pool->n_kv_heads <= kMaxGroup &&
            n_q >= 0 && n_seqs >= 0 && max_q > 0 &&
            static_cast<long long>(max_q) * (n_heads / pool->n_kv_heads) <= kMaxRows && prefix_len >= 0 &&
-           static_cast<long long>(n_q) * (n_heads / pool->n_kv_heads) <= kMaxBatchRows;
+           static_cast<long long>(n_q) * (n_heads / pool->n_kv_heads) <= kMaxBatchRows &&
+           static_cast<long long>(n_seqs) * max_q * n_heads <= INT_MAX;
 }
 
 // Lays the workspace out from its start; returns its size.

@@ -33,7 +33,8 @@ struct PagedArgs {
 
 constexpr float kShift = 8.0f;     // the weights' largest is about 2^8: fp16 then reaches to 2^-32 of it
 constexpr int kMaxBlocks = 640;    // of the own-pages kernel: at least 4 a multiprocessor
-constexpr int kMinPages = 8;       // a block's smallest share of pages
+constexpr int kSetup = 4;          // what a strip costs beside its pages, in pages
+constexpr int kMinUnits = 8;       // a block's smallest share
 
 // Rows of sequence b and its own tokens, whatever the arrays hold.
 struct SeqShape {
