@@ -96,6 +96,25 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
     }
 }
 
+// The same onto zeros.
+template <bool F16>
+__device__ __forceinline__ void mma16816_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                             uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (F16) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    } else {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    }
+}
+
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -157,9 +176,68 @@ __device__ __forceinline__ void block_scan(long long mine, long long* warp_sums,
     }
 }
 
+// Units of a strip; one without pages has one all the same, so that a block sees to its rows.
+__device__ __forceinline__ int strip_units(int pages) { return max(pages, 1) + kSetup; }
+
 template <int NT>
 __device__ __forceinline__ int row_groups(const SeqShape& s, int group) {
     return (s.rows * group + 8 * NT - 1) / (8 * NT);
+}
+
+// Joins one row's n parts and writes its head, by one warp: a lane looks up a part's weight and place
+// (part_of(i, ml, o)), then all lanes add the part's sums, several parts on their way at once. The
+// order is the parts', whoever joins them.
+template <int D, typename PartOf>
+__device__ __forceinline__ void join_row(int n, PartOf part_of, uint16_t* out, int f16) {
+    constexpr int V = D / 32;
+    const int lane = threadIdx.x & 31;
+    float top = -INFINITY, sum = 0.0f;  // sum: this lane's parts
+    float y[V] = {};
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        const float* o = nullptr;
+        if (i0 + lane < n) {
+            const float2* p;
+            part_of(i0 + lane, p, o);
+            ml = __ldcg(p);
+        }
+        const float top_new = fmaxf(top, warp_max(ml.x));
+        const float back = top_new == top ? 1.0f : ex2(top - top_new);
+        const float f = ml.x == top_new ? 1.0f : ex2(ml.x - top_new);
+        top = top_new;
+        sum = fmaf(ml.y, f, sum * back);
+#pragma unroll
+        for (int d = 0; d < V; ++d) y[d] *= back;
+        const int here = min(32, n - i0);
+#pragma unroll 8
+        for (int x = 0; x < here; ++x) {
+            const float* ox = reinterpret_cast<const float*>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), x));
+            const float fx = __shfl_sync(0xffffffffu, f, x);
+            float z[V];
+            if constexpr (V == 4) *reinterpret_cast<float4*>(z) = __ldcg(reinterpret_cast<const float4*>(ox + lane * V));
+            else *reinterpret_cast<float2*>(z) = __ldcg(reinterpret_cast<const float2*>(ox + lane * V));
+#pragma unroll
+            for (int d = 0; d < V; ++d) y[d] = fmaf(z[d], fx, y[d]);
+        }
+    }
+    sum = warp_sum(sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing is zeros
+    uint32_t z[V / 2];
+#pragma unroll
+    for (int d = 0; d < V; d += 2) z[d / 2] = pack2_out(y[d] * inv, y[d + 1] * inv, f16);
+    if constexpr (V == 4) *reinterpret_cast<uint2*>(out + lane * V) = make_uint2(z[0], z[1]);
+    else *reinterpret_cast<uint32_t*>(out + lane * V) = z[0];
+}
+
+template <int NT>
+__device__ __forceinline__ long long seq_units(const PagedArgs& a, const SeqShape& s) {
+    return static_cast<long long>(a.n_kv) * row_groups<NT>(s, a.group) * strip_units(seq_pages(s));
+}
+
+// Units of one block's run.
+__device__ __forceinline__ long long run_length(long long total, unsigned blocks) {
+    return max(static_cast<long long>(kMinUnits), (total + blocks - 1) / static_cast<long long>(blocks));
 }
 
 template <int D, bool E4M3, int NT>
@@ -193,28 +271,12 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
     // This block's run of units.
     const int per_thread = (a.n_seqs + kThreads - 1) / kThreads;
     const int b0 = min(tid * per_thread, a.n_seqs), b1 = min(b0 + per_thread, a.n_seqs);
-    auto units = [&](int b) {
-        const SeqShape s = seq_shape(a, b);
-        const int pages = seq_pages(s);
-        return pages ? static_cast<long long>(a.n_kv) * row_groups<NT>(s, a.group) * (pages + kSetup) : 0;
-    };
+    auto units = [&](int b) { return seq_units<NT>(a, seq_shape(a, b)); };
     long long mine = 0, before, total;
     for (int b = b0; b < b1; ++b) mine += units(b);
     block_scan(mine, scan_s, before, total);
-    const long long per = max(static_cast<long long>(kMinUnits),
-                              (total + gridDim.x - 1) / static_cast<long long>(gridDim.x));
+    const long long per = run_length(total, gridDim.x);
     const long long start = per * blockIdx.x, end = min(total, start + per);
-    if (blockIdx.x == 0) {
-        long long x = before;
-        for (int b = b0; b < b1; ++b) {
-            a.first_unit[b] = x;
-            x += units(b);
-        }
-        if (tid == 0) {
-            a.first_unit[a.n_seqs] = total;
-            a.first_unit[a.n_seqs + 1] = per;
-        }
-    }
     if (start >= end) {
         pdl_wait();
         return;
@@ -235,18 +297,22 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
     while (pos < end) {
         const SeqShape s = seq_shape(a, b);
         const int pages = seq_pages(s), groups = row_groups<NT>(s, a.group);
-        const long long all = pages ? static_cast<long long>(a.n_kv) * groups * (pages + kSetup) : 0;
+        const int each = strip_units(pages);
+        const long long all = static_cast<long long>(a.n_kv) * groups * each;
         if (pos >= seq_first + all) {
             seq_first += all;
             ++b;
             continue;
         }
-        const long long strip = (pos - seq_first) / (pages + kSetup);  // (head, row group)
-        const long long u0 = pos - seq_first - strip * (pages + kSetup);
-        const long long u1 = min(static_cast<long long>(pages) + kSetup, u0 + (end - pos));
-        const int p0 = static_cast<int>(max(0LL, u0 - kSetup)), p1 = static_cast<int>(u1 - kSetup);
-        pos += u1 - u0;
-        if (p1 <= 0) continue;  // the run ends before the strip's first page
+        const long long strip = (pos - seq_first) / each;  // (head, row group)
+        const long long strip_first = seq_first + strip * each;
+        const long long u1 = min(strip_first + each, end);
+        // This block's pages of it: all of them, or the run's beginning or end cuts them.
+        const int p0 = static_cast<int>(max(0LL, pos - strip_first - kSetup));
+        const int p1 = min(pages, static_cast<int>(u1 - strip_first) - kSetup);
+        const bool touched = u1 - strip_first > kSetup;
+        pos = u1;
+        if (!touched) continue;  // the run ends in front of the strip's first page
         const int h = static_cast<int>(strip / groups), rg = static_cast<int>(strip % groups);
         const int r_base = rg * ROWS;
         const int n_rows = min(ROWS, s.rows * a.group - r_base);
@@ -255,6 +321,7 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
         const int32_t* table = a.table + static_cast<size_t>(b) * a.table_stride;
         const int steps = p1 - p0 > warp ? (p1 - p0 - warp + kWarps - 1) / kWarps : 0;
         int ids = 0;
+        uint32_t fill = ring, page_s = ring;  // the ring's next page to fill, to use
         unsigned good = 0;  // of the last 32 steps looked up: whether the page is in the pool
         auto start_page = [&](int it) {  // in order: 0, 1, 2, ...
             if ((it & 31) == 0) {
@@ -266,7 +333,8 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
             good = good << 1 | in;
             // A page that is not there is page 0 in its place, whose keys are masked.
             const size_t row = (static_cast<size_t>(in ? page : 0) * a.n_kv + h) * kPageTokens;
-            const uint32_t to = ring + (it % STAGES) * L::kPage;
+            const uint32_t to = fill;
+            fill = fill == ring + (STAGES - 1) * L::kPage ? ring : fill + L::kPage;
             const uint8_t* kp = static_cast<const uint8_t*>(a.k) + row * ROW;
             const uint8_t* vp = static_cast<const uint8_t*>(a.v) + row * ROW;
 #pragma unroll
@@ -343,13 +411,13 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
         }
         const int tail_key = s.len - s.rows + r_base / a.group + 1;  // seen by every row below it
 
-        float m[NT][2], neg[NT][2], l[NT][2], o[NT][MT][4];
+        float m[NT][2], lim[NT][2], neg[NT][2], l[NT][2], o[NT][MT][4];  // lim = m + kGrow, neg = kShift - m
         int r_v = -1000;  // power of two that o is relative to
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                m[n][x] = -INFINITY;
+                m[n][x] = lim[n][x] = -INFINITY;
                 neg[n][x] = kShift;
                 l[n][x] = 0.0f;
             }
@@ -365,7 +433,6 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
             const bool there = good >> (min(it + STAGES - 2, steps - 1) - it) & 1;
             if (it + STAGES - 1 < steps) start_page(it + STAGES - 1);
             copy_commit();
-            const uint32_t page_s = ring + (it % STAGES) * L::kPage;
             constexpr int SW = PIECES < 8 ? PIECES - 1 : 7;
             uint32_t kr[2][KW], vr[4][VW], ex[2] = {0, 0};
 #pragma unroll
@@ -379,13 +446,7 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
                 ex[0] = lds_u16(page_s + 2 * kPageTokens * ROW + g * 2);
                 ex[1] = lds_u16(page_s + 2 * kPageTokens * ROW + g * 2 + 16);
             }
-            // Scores: two chains of products, so that one is not a wait for the other.
-            float sc[NT][2][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sc[n][0][i] = sc[n][1][i] = 0.0f;
-            }
+            float sc[NT][4];
 #pragma unroll
             for (int k = 0; k < MT; ++k) {
                 uint32_t f[4];
@@ -402,7 +463,8 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    mma16816<E4M3>(sc[n][k & 1], f[0], f[1], f[2], f[3], qw[n][2 * k], qw[n][2 * k + 1]);
+                    if (k == 0) mma16816_new<E4M3>(sc[n], f[0], f[1], f[2], f[3], qw[n][0], qw[n][1]);
+                    else mma16816<E4M3>(sc[n], f[0], f[1], f[2], f[3], qw[n][2 * k], qw[n][2 * k + 1]);
                 }
             }
             const bool tail = !there || key0 + kPageTokens > tail_key;
@@ -413,11 +475,11 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float x = (sc[n][0][i] + sc[n][1][i]) * c_col[n][i & 1];
+                    float x = sc[n][i] * c_col[n][i & 1];
                     if constexpr (E4M3) x *= __uint_as_float((ex[i >> 1] & 0xffu) << 23);  // 2^(byte - 127)
                     if (tail && (!there || key0 + g + 8 * (i >> 1) >= seen[n][i & 1])) x = -INFINITY;
                     p[n][i] = x;
-                    grow |= x > m[n][i & 1] + kGrow;
+                    grow |= x > lim[n][i & 1];
                 }
             }
             int v_top = 0;
@@ -446,6 +508,7 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
                         const float m_new = fmaxf(m[n][x], mx);
                         f[x] = m_new == m[n][x] ? 1.0f : ex2(m[n][x] - m_new);
                         m[n][x] = m_new;
+                        lim[n][x] = m_new + kGrow;
                         neg[n][x] = kShift - (m_new == -INFINITY ? 0.0f : m_new);
                         l[n][x] *= f[x];
                         f[x] *= fv;
@@ -462,8 +525,9 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
             uint32_t pb[NT][2], pl[NT][2];  // P^T as the B operand (and its low half)
             float vf[2] = {1.0f, 1.0f};
             if constexpr (E4M3) {
-                vf[0] = pow2(static_cast<int>(ex[0] >> 8) - r_v);
-                vf[1] = pow2(static_cast<int>(ex[1] >> 8) - r_v);
+                // 2^(byte - r_v), at most 2^kGrowV; below 2^-126 it is 0.
+                vf[0] = __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(ex[0] >> 8) - r_v + 127, 0)) << 23);
+                vf[1] = __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(ex[1] >> 8) - r_v + 127, 0)) << 23);
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -553,6 +617,7 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
                     }
                 }
             }
+            page_s = page_s == ring + (STAGES - 1) * L::kPage ? ring : page_s + L::kPage;
         }
 
         // Join the warps.
@@ -633,87 +698,67 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
     pdl_wait();
 }
 
-// Joins a row's parts: those of its sequence's own pages, where blocks cut them or a prefix adds to
-// them, and the prefix's. A warp a row: a lane looks up a part's weight and place, then all lanes add
-// the part's sums, several parts on their way at once.
+// Joins the rows that have several parts: those of the prefix, and of the sequence's own pages one
+// where a block did the whole strip and one a block where they cut it. A warp a row. It finds the
+// blocks' runs from the lengths again, while own_pages_kernel is still at work.
 template <int D, int NT>
-__global__ void __launch_bounds__(kThreads) join_kernel(const PagedArgs a) {
-    constexpr int ROWS = 8 * NT, V = D / 32;
-    const int lane = threadIdx.x & 31, most = a.max_q * a.group;
+__global__ void __launch_bounds__(kThreads) join_kernel(const PagedArgs a, const unsigned blocks) {
+    constexpr int ROWS = 8 * NT;
+    const int most = a.max_q * a.group, lane = threadIdx.x & 31;
     const long long w = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
     const int r = static_cast<int>(w % most), h = static_cast<int>(w / most % a.n_kv);
     const long long b = w / most / a.n_kv;
-    if (b >= a.n_seqs) return;
+    // Every block waits, also one with nothing to do: what comes after this grid comes after both.
+    if (b >= a.n_seqs) {
+        pdl_wait();
+        return;
+    }
     const SeqShape s = seq_shape(a, static_cast<int>(b));
-    if (r >= s.rows * a.group) return;
-    const int pages = seq_pages(s), groups = row_groups<NT>(s, a.group);
+    long long before = 0, total = 0;
+    for (int i = lane; i < a.n_seqs; i += 32) {
+        const long long u = seq_units<NT>(a, seq_shape(a, i));
+        total += u;
+        if (i < b) before += u;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    const int each = strip_units(seq_pages(s)), groups = row_groups<NT>(s, a.group);
+    const long long per = run_length(total, blocks);
+    const long long first = before + (static_cast<long long>(h) * groups + r / ROWS) * each;
+    const long long c0 = (first + kSetup) / per, c1 = (first + each - 1) / per;
+    const int own = static_cast<int>(c1 - c0 + 1);
     pdl_wait();
-    const long long per = a.first_unit[a.n_seqs + 1];
-    const long long u0 = a.first_unit[b] + kSetup +
-                         (static_cast<long long>(h) * groups + r / ROWS) * (pages + kSetup);
-    const long long c0 = u0 / per, c1 = pages ? (u0 + pages - 1) / per : c0 - 1;
-    if (a.prefix_len == 0 && c0 == c1) return;  // finished by its block
-    const int own = static_cast<int>(c1 - c0 + 1), n = own + a.prefix_splits;
+    if (r >= s.rows * a.group || (own == 1 && a.prefix_len == 0)) return;  // no row; finished by its block
     const size_t row = h * static_cast<size_t>(a.prefix_rows) + static_cast<size_t>(s.row0) * a.group + r;
     const size_t split = static_cast<size_t>(a.n_kv) * a.prefix_rows;
-    float top = -INFINITY, sum = 0.0f;  // sum: this lane's parts
-    float y[V] = {};
-    for (int i0 = 0; i0 < n; i0 += 32) {
-        const int i = i0 + lane;
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        const float* o = nullptr;
-        if (i < n) {
-            const float2* p;
+    join_row<D>(
+        own + a.prefix_splits,
+        [&](int i, const float2*& ml, const float*& o) {
             if (i >= own) {
                 const size_t at = (i - own) * split + row;
-                p = a.prefix_ml + at;
+                ml = a.prefix_ml + at;
                 o = a.prefix_o + at * D;
             } else if (own == 1) {
-                p = a.whole_ml + row;
+                ml = a.whole_ml + row;
                 o = a.whole_o + row * D;
             } else {
                 const size_t at = ((c0 + i) * 2 + (i == 0)) * ROWS + r % ROWS;
-                p = a.own_ml + at;
+                ml = a.own_ml + at;
                 o = a.own_o + at * D;
             }
-            ml = *p;
-        }
-        const float top_new = fmaxf(top, warp_max(ml.x));
-        const float back = top_new == top ? 1.0f : ex2(top - top_new);
-        const float f = ml.x == top_new ? 1.0f : ex2(ml.x - top_new);
-        top = top_new;
-        sum = fmaf(ml.y, f, sum * back);
-#pragma unroll
-        for (int d = 0; d < V; ++d) y[d] *= back;
-        const int here = min(32, n - i0);
-#pragma unroll 8
-        for (int x = 0; x < here; ++x) {
-            const float* ox = reinterpret_cast<const float*>(
-                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), x));
-            const float fx = __shfl_sync(0xffffffffu, f, x);
-            float z[V];
-            if constexpr (V == 4) *reinterpret_cast<float4*>(z) = *reinterpret_cast<const float4*>(ox + lane * V);
-            else *reinterpret_cast<float2*>(z) = *reinterpret_cast<const float2*>(ox + lane * V);
-#pragma unroll
-            for (int d = 0; d < V; ++d) y[d] = fmaf(z[d], fx, y[d]);
-        }
-    }
-    sum = warp_sum(sum);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint16_t* out = static_cast<uint16_t*>(a.out) + (s.row0 + r / a.group) * a.out_stride +
-                    (h * a.group + r % a.group) * D + lane * V;
-    uint32_t z[V / 2];
-#pragma unroll
-    for (int d = 0; d < V; d += 2) z[d / 2] = pack2_out(y[d] * inv, y[d + 1] * inv, a.f16);
-    if constexpr (V == 4) *reinterpret_cast<uint2*>(out) = make_uint2(z[0], z[1]);
-    else *reinterpret_cast<uint32_t*>(out) = z[0];
+        },
+        static_cast<uint16_t*>(a.out) + (s.row0 + r / a.group) * a.out_stride + (h * a.group + r % a.group) * D,
+        a.f16);
 }
 
 template <int D, bool E4M3, int NT>
 void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
     const long long groups = (static_cast<long long>(a.max_q) * a.group + 8 * NT - 1) / (8 * NT);
     // No more blocks than the table's width could fill.
-    const long long most = (static_cast<long long>(a.n_seqs) * a.n_kv * (a.table_stride + kSetup) * groups +
+    const long long most = (static_cast<long long>(a.n_seqs) * a.n_kv * (std::max(a.table_stride, 1) + kSetup) * groups +
                             kMinUnits - 1) / kMinUnits;
     const int grid = static_cast<int>(std::max(
         1LL, std::min({most, static_cast<long long>(sms) * Shape<E4M3, NT>::kBlocks, static_cast<long long>(kMaxBlocks)})));
@@ -722,7 +767,7 @@ void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
     launch_dep(a.prefix_len > 0, own_pages_kernel<D, E4M3, NT>, dim3(grid), dim3(kThreads), bytes, s, a);
     const long long rows = static_cast<long long>(a.n_seqs) * a.n_kv * a.max_q * a.group;
     launch_dep(true, join_kernel<D, NT>, dim3(static_cast<unsigned>((rows + kWarps - 1) / kWarps)),
-               dim3(kThreads), 0, s, a);
+               dim3(kThreads), 0, s, a, static_cast<unsigned>(grid));
 }
 
 template <int D, bool E4M3>
@@ -752,7 +797,6 @@ size_t lay_out(PagedArgs& a, uint8_t* base, int head_dim) {
         return p;
     };
     const size_t rows = a.max_q * a.group <= 8 ? 8 : 16;
-    a.first_unit = reinterpret_cast<long long*>(take((static_cast<size_t>(a.n_seqs) + 2) * 8));
     a.own_ml = reinterpret_cast<float2*>(take(kMaxBlocks * 2 * rows * 8));
     a.own_o = reinterpret_cast<float*>(take(kMaxBlocks * 2 * rows * head_dim * 4));
     if (a.prefix_len > 0) {

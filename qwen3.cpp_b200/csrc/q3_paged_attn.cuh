@@ -21,7 +21,6 @@ struct PagedArgs {
     int f16;         // q and out are fp16 (else bf16)
     // Workspace. Partial results are in fp32: o = sum p v and (m, l) = (max of the scores in units of
     // log2, sum p), p = 2^(score - m + kShift).
-    long long* first_unit;  // [n_seqs + 2]: units before each sequence, all of them, units a block
     float* own_o;           // [blocks][2][8 * tiles][head_dim]
     float2* own_ml;         // [blocks][2][8 * tiles]
     float* whole_o;         // [n_kv][prefix_rows][head_dim]: with a prefix, own parts that were not cut
