@@ -7,12 +7,13 @@
 // differences are exact in 64 bits, and a running sum over 1.5e5 values is within ~1e-13 there, so the
 // drawn token does not hang on the order of the additions.
 //
-// Only the accepted drafts' single values and one row of p and q are read. A cluster of up to 8 CTAs
+// Only the accepted drafts' single values and one row of p and q are read. A cluster of up to 16 CTAs
 // takes a sequence: every CTA finds the accepted count (a few gathers), sums its share of the row, one
 // contiguous piece a warp, and passes its sum to the others' shared memory; one cluster barrier later
 // each knows the total and the sums before it, and the one warp in whose piece the goal falls goes
-// through that piece again (from cache) for the index. One launch, no workspace. Bound by HBM for
-// many sequences (2 * vocab * 4 bytes each), by latency for one: TIMES.
+// through that piece again (from cache) for the index. One launch, no workspace. With vocab 151936, 64
+// sequences of 5 drafts take 24 us (78 MB, 3.2 TB/s: 14 us of them the reading, the rest the chain of
+// dependent steps around it), one of 4 drafts 7.1 us, all latency.
 #include <algorithm>
 #include <climits>
 
@@ -35,9 +36,10 @@ struct VerifyArgs {
     int max_drafts, vocab, ctas;  // ctas: of a sequence's cluster
 };
 
-constexpr int kVerifyThreads = 512;
+constexpr int kVerifyThreads = 512;   // at most
 constexpr int kVerifyWarps = kVerifyThreads / 32;
-constexpr int kMaxCtas = 8;      // the portable cluster size
+constexpr int kUnroll = 2;           // 16-byte loads of p, and of q, that a lane has on their way (5: 6% slower)
+constexpr int kMaxCtas = 16;       // of a cluster
 constexpr int kLeastShare = 4096;  // values that are worth a CTA: below, its start costs more than it reads
 
 __device__ __forceinline__ float share(float x) { return x > 0.0f ? x : 0.0f; }  // NaN is 0
@@ -107,38 +109,46 @@ __device__ __forceinline__ void for_row(const Row& row, int i0, int i1, F f) {
     }
 }
 
-template <int V>
+// Sum and last share of [i0, i1), for all lanes of the warp. V sums at once: a 64-bit addition takes
+// tens of cycles.
+template <int V, int UNROLL>
 __device__ __forceinline__ Piece sum_piece(const Row& row, int i0, int i1) {
-    double sum = 0.0;
+    double part[V] = {};
     int last = -1;
-    for_row<V, 4>(row, i0, i1, [&](int i, const double (&r)[V]) {
+    for_row<V, UNROLL>(row, i0, i1, [&](int i, const double (&r)[V]) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            sum += r[k];
+            part[k] += r[k];
             if (r[k] > 0.0) last = i + k;
         }
     });
+    double sum = V == 4 ? (part[0] + part[1 % V]) + (part[2 % V] + part[3 % V]) : part[0];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return {sum, static_cast<int>(__reduce_max_sync(0xffffffffu, last))};
 }
 
-// First index of [i0, i1) at which the running sum, `before` in front of it, passes goal; `last` if the
-// roundings of another order keep it from that.
-template <int V>
-__device__ __forceinline__ int find_in_piece(const Row& row, int i0, int i1, double before, double goal, int last) {
-    int found = INT_MAX;
+// The lanes' running sum.
+__device__ __forceinline__ double running_sum(double x) {
     const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+
+constexpr int kScan = 128;  // values that one warp scans
+
+// First index of [i0, i1), at most kScan values, at which the running sum, `before` in front of it,
+// passes goal; `last` if the roundings of another order keep it from that.
+template <int V>
+__device__ __forceinline__ int scan(const Row& row, int i0, int i1, double before, double goal, int last) {
+    int found = INT_MAX;
     for_row<V, 1>(row, i0, i1, [&](int i, const double (&r)[V]) {
-        double mine = 0.0;
-#pragma unroll
-        for (int k = 0; k < V; ++k) mine += r[k];
-        double run = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double x = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += x;
-        }
+        const double mine = V == 4 ? (r[0] + r[1 % V]) + (r[2 % V] + r[3 % V]) : r[0];
+        const double run = running_sum(mine);
         double c = before + (run - mine);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -151,103 +161,129 @@ __device__ __forceinline__ int find_in_piece(const Row& row, int i0, int i1, dou
     return found == INT_MAX ? last : found;
 }
 
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyArgs a) {
     __shared__ Piece warps_s[kVerifyWarps];
     __shared__ Piece ctas_s[2][kMaxCtas];  // written by the cluster's CTAs, per attempt
     __shared__ int accepted_s;
     const int b = blockIdx.x / a.ctas, rank = blockIdx.x % a.ctas;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n_warps = blockDim.x >> 5;
     const int32_t* tok = a.draft_tokens + static_cast<size_t>(b) * a.max_drafts;
     int count = a.max_drafts;
-    if (a.max_drafts && a.n_drafts) count = min(max(a.n_drafts[b], 0), a.max_drafts);
+    if (a.max_drafts && a.n_drafts) count = a.n_drafts[b];
+    const float u_sample = a.u_sample[b];  // needed last, on its way first
     if (warp == 0) {
-        int n = count;
-        for (int j0 = 0; j0 < count; j0 += 32) {
-            const int j = j0 + lane;
-            bool good = j < count;
-            if (good) {
-                const int t = tok[j];
-                const double u = a.u_accept[static_cast<size_t>(b) * a.max_drafts + j];
-                good = t >= 0 && t < a.vocab;
-                if (good) {
-                    const double p = a.target[b * a.t_seq + j * a.t_row + t];
-                    const float q = a.draft ? a.draft[b * a.d_seq + j * a.d_row + t] : 1.0f;
-                    good = u * share(q) < p;
-                }
+        int n = INT_MAX;
+        for (int j0 = 0; j0 < a.max_drafts && n == INT_MAX; j0 += 32) {
+            const int j = min(j0 + lane, a.max_drafts - 1);
+            const int t = tok[j];  // on its way with the count
+            const double u = a.u_accept[static_cast<size_t>(b) * a.max_drafts + j];
+            bool good = j0 + lane < min(count, a.max_drafts);
+            if (good && t >= 0 && t < a.vocab) {
+                const double p = a.target[b * a.t_seq + j * a.t_row + t];
+                const float q = a.draft ? a.draft[b * a.d_seq + j * a.d_row + t] : 1.0f;
+                good = u * share(q) < p;
+            } else {
+                good = false;
             }
             const unsigned bad = __ballot_sync(0xffffffffu, !good);
-            if (bad) {
-                n = min(n, j0 + __ffs(bad) - 1);
-                break;
-            }
+            if (bad) n = j0 + __ffs(bad) - 1;
         }
+        n = min(n, a.max_drafts);
         if (lane == 0) accepted_s = n;
     }
     __syncthreads();
+    count = min(max(count, 0), a.max_drafts);
     const int n = accepted_s;
     Row row;
     row.p = a.target + b * a.t_seq + n * a.t_row;
     row.q = n < count && a.draft ? a.draft + b * a.d_seq + n * a.d_row : nullptr;
     row.one = n < count && !a.draft ? tok[n] : -1;
     // Pieces start on multiples of 4, so that they are as aligned as the row.
-    const long long pieces = static_cast<long long>(a.ctas) * kVerifyWarps;
+    const long long pieces = static_cast<long long>(a.ctas) * n_warps;
     const int per = static_cast<int>(((a.vocab + pieces - 1) / pieces + 3) / 4 * 4);
-    const int i0 = static_cast<int>(min(static_cast<long long>(a.vocab), (rank * kVerifyWarps + warp) * static_cast<long long>(per)));
+    const int i0 = static_cast<int>(min(static_cast<long long>(a.vocab), (rank * n_warps + warp) * static_cast<long long>(per)));
     const int i1 = static_cast<int>(min(static_cast<long long>(a.vocab), i0 + static_cast<long long>(per)));
     const bool vec = ((reinterpret_cast<uintptr_t>(row.p) | reinterpret_cast<uintptr_t>(row.q)) & 15) == 0;
-    Piece mine{};
-    double total = 0.0, before = 0.0, after = 0.0;
+    // The sums before this CTA's share and up to its end, added up in one order everywhere, so that one's
+    // end is the next one's beginning to the bit and every goal lies in exactly one.
+    double total = 0.0, cta_before = 0.0, cta_after = 0.0;
     int last = -1;
     for (int attempt = 0; attempt < 2; ++attempt) {
-        mine = vec ? sum_piece<4>(row, i0, i1) : sum_piece<1>(row, i0, i1);
+        const Piece mine = vec ? sum_piece<4, kUnroll>(row, i0, i1) : sum_piece<1, kUnroll>(row, i0, i1);
         if (lane == 0) warps_s[warp] = mine;
         __syncthreads();
-        if (tid < a.ctas) {
+        if (warp == 0) {
             Piece all{0.0, -1};
+            if (lane < n_warps) all = warps_s[lane];
 #pragma unroll
-            for (int w = 0; w < kVerifyWarps; ++w) {
-                all.sum += warps_s[w].sum;
-                all.last = max(all.last, warps_s[w].last);
+            for (int o = 16; o > 0; o >>= 1) all.sum += __shfl_xor_sync(0xffffffffu, all.sum, o);
+            all.last = __reduce_max_sync(0xffffffffu, all.last);
+            if (lane < a.ctas) {
+                uint32_t to;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                             : "=r"(to)
+                             : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(&ctas_s[attempt][rank]))), "r"(lane));
+                asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(all.sum) : "memory");
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 8), "r"(all.last) : "memory");
             }
-            uint32_t to;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                         : "=r"(to)
-                         : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(&ctas_s[attempt][rank]))), "r"(tid));
-            asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(all.sum) : "memory");
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 8), "r"(all.last) : "memory");
+            __syncwarp();
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        total = before = 0.0;
+        total = 0.0;
         last = -1;
         for (int c = 0; c < a.ctas; ++c) {
-            if (c == rank) before = total;
+            if (c == rank) cta_before = total;
             total += ctas_s[attempt][c].sum;
+            if (c == rank) cta_after = total;
             last = max(last, ctas_s[attempt][c].last);
         }
-        // This piece's two ends, added up in one order everywhere, so that one's end is the next one's
-        // beginning to the bit and every goal lies in exactly one.
-        double in_cta = 0.0;
-        for (int w = 0; w < warp; ++w) in_cta += warps_s[w].sum;
-        after = before + (in_cta + mine.sum);
-        before += in_cta;
         if (total > 0.0) break;
         row.q = nullptr;  // nothing is left over: the target's own row
         row.one = -1;
         __syncthreads();
     }
-    const double goal = fmax(static_cast<double>(a.u_sample[b]) * total, 0.0);
+    const double goal = fmax(static_cast<double>(u_sample) * total, 0.0);
     int32_t* out = a.tokens + static_cast<size_t>(b) * (a.max_drafts + 1);
-    if (before <= goal && goal < after) {
-        const int at = vec ? find_in_piece<4>(row, i0, i1, before, goal, mine.last)
-                           : find_in_piece<1>(row, i0, i1, before, goal, mine.last);
-        if (lane == 0) out[n] = at;
+    if (cta_before <= goal && goal < cta_after) {
+        // The token lies in this CTA's share: its warps cut the warp's piece it lies in among them until
+        // one warp can scan what is left (one round for 1e5 values).
+        int j0 = i0 - warp * per, j1 = static_cast<int>(min(static_cast<long long>(a.vocab), j0 + static_cast<long long>(per) * n_warps));
+        int step = per;
+        double base = cta_before;
+        int at = -1;
+        while (true) {
+            // The piece among [j0, j1)'s that the goal lies in; the last with a share if roundings put it
+            // behind all of them. Every warp works it out, a lane a piece.
+            Piece x{0.0, -1};
+            if (lane < n_warps) x = warps_s[lane];
+            const double up_to = running_sum(x.sum);
+            const unsigned has = __ballot_sync(0xffffffffu, x.last >= 0);
+            const unsigned past = __ballot_sync(0xffffffffu, x.last >= 0 && goal < base + up_to);
+            const int pick = past ? __ffs(past) - 1 : 31 - __clz(has | 1u);
+            const int pick_last = __shfl_sync(0xffffffffu, x.last, pick);
+            const double below = __shfl_sync(0xffffffffu, base + (up_to - x.sum), pick);
+            j0 += pick * step;
+            j1 = min(j1, j0 + step);
+            base = below;
+            if (j1 - j0 <= kScan) {
+                if (warp == 0) at = vec ? scan<4>(row, j0, j1, base, goal, pick_last) : scan<1>(row, j0, j1, base, goal, pick_last);
+                break;
+            }
+            step = ((j1 - j0 + n_warps - 1) / n_warps + 3) / 4 * 4;
+            const int k0 = min(j1, j0 + warp * step), k1 = min(j1, k0 + step);
+            const Piece mine = vec ? sum_piece<4, 1>(row, k0, k1) : sum_piece<1, 4>(row, k0, k1);
+            __syncthreads();
+            if (lane == 0) warps_s[warp] = mine;
+            __syncthreads();
+        }
+        if (tid == 0) out[n] = at;
     }
     if (rank == 0) {
         if (tid == 0) {
             a.n_accepted[b] = n;
             if (!(goal < total)) out[n] = max(last, 0);
         }
-        for (int j = tid; j <= a.max_drafts; j += kVerifyThreads) {
+        for (int j = tid; j <= a.max_drafts; j += blockDim.x) {
             if (j != n) out[j] = j < n ? tok[j] : -1;
         }
     }
@@ -284,15 +320,24 @@ extern "C" q3_status q3_verify_drafts(int32_t* tokens, int32_t* n_accepted, cons
         }
         const q3::OnDevice on({tokens, n_accepted, target, draft, max_drafts ? draft_tokens : nullptr,
                                n_drafts, max_drafts ? u_accept : nullptr, u_sample});
-        // As many CTAs as have kLeastShare values each, a power of two.
+        // As many CTAs as have kLeastShare values each, a power of two: up to 16 for up to 4 sequences (a
+        // multiprocessor reads about 40 GB/s from L2, so one sequence's row takes 7.1 us on 16 and 8.3
+        // on 8), else up to 8 (clusters of 16 find room less easily: 64 sequences 36 us against 24).
+        const int most = n_seqs <= 4 ? q3::kMaxCtas : q3::kMaxCtas / 2;
         int ctas = 1;
-        while (ctas < q3::kMaxCtas && vocab >= 2 * ctas * q3::kLeastShare) ctas *= 2;
+        while (ctas < most && vocab >= 2 * ctas * q3::kLeastShare) ctas *= 2;
         if (n_seqs > INT_MAX / ctas) throw std::invalid_argument("draft verification: size out of range");
         const q3::VerifyArgs a{tokens, n_accepted, target, draft, draft_tokens, n_drafts, u_accept,
                                u_sample, t_seq, t_row, d_seq, d_row, max_drafts, vocab, ctas};
+        if (ctas > 8) {
+            Q3_CUDA(cudaFuncSetAttribute(q3::verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        }
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(n_seqs) * ctas);
-        cfg.blockDim = dim3(q3::kVerifyThreads);
+        // With more CTAs than multiprocessors, smaller ones, so that they are all resident at once (64
+        // sequences: 24 us against 28); else the larger, whose lanes go round less often.
+        cfg.blockDim = dim3(static_cast<long long>(n_seqs) * ctas > on.sm_count() ? q3::kVerifyThreads / 2
+                                                                                 : q3::kVerifyThreads);
         cfg.stream = static_cast<cudaStream_t>(stream);
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
