@@ -7,7 +7,7 @@
 // that the tensor cores work on one while the softmax of the other runs:
 //   PAIR  more than 128 rows: two row tiles, each over all of the CTA's key tiles; K and V are brought
 //         in once for both
-//   SOLO  one row tile: one stream over the even key tiles, one over the odd ones (a part each)
+//   SOLO  one row tile: one stream over the even key tiles, one over the odd ones, added at the end
 // Per stream and key tile:
 //   issuer   S = Q . K^T                  tcgen05.mma, M = N = 128, into TMEM
 //   softmax  P = 2^(S c - m + kShift)      one thread a row; P replaces S in TMEM, as fp16 (e4m3 pool) or
@@ -16,13 +16,15 @@
 // O stays in TMEM. The running maximum moves only when a score passes it by more than 2^kGrow; then
 // the row's O is read, scaled and written back (rare after the first tile).
 //
-// Four warps bring the tiles in: 16-byte loads one tile ahead, written in the operands' 128-byte
-// swizzled layout. e4m3 codes become fp16 there, exactly, times 2^(byte - largest byte of the CTA's
-// keys): exact down to 2^-15 of the largest row, below that to 2^-25 of its unit. One factor in front
-// of the scores and one behind the sums then stand for all bytes.
+// Four warps bring the tiles in by cp.async, ahead of their use, into the operands' 128-byte swizzled
+// layout: bf16 directly; e4m3 codes by way of a ring of raw tiles, from which they become fp16, exactly,
+// times 2^(byte - largest byte of the CTA's keys): exact down to 2^-15 of the largest row, below that
+// to 2^-25 of its unit. One factor in front of the scores and one behind the sums then stand for all
+// bytes.
 //
-// Warps: 0-3 and 4-7 softmax of stream 0 and 1, 8-11 loaders, 12 issuer. Every wait is bounded; one
-// that gives up ends the CTA's loops and leaves NaN in its parts.
+// Warps: 0-3 and 4-7 softmax of stream 0 and 1 (a row's 128 scores stay in registers, hence the uneven
+// split of the registers), 8-11 loaders, 12 issuer. Every wait is bounded; one that gives up ends the
+// CTA's loops and leaves NaN in its parts.
 #include <algorithm>
 
 #include "q3_paged_attn.cuh"
@@ -37,22 +39,27 @@ using namespace sm100;
 constexpr int kRowTile = 128, kKeyTile = 128;
 constexpr int kPagesPerTile = kKeyTile / kPageTokens;
 constexpr int kMaxTiles = 512;      // key tiles of one CTA (the size of its list of good pages)
-constexpr int kPrefixThreads = 416;
+constexpr int kPrefixThreads = 512;
+constexpr int kManyRegs = 192, kFewRegs = 64;  // 8 warps each: 512 threads are launched with 128
 constexpr float kGrow = 6.0f;       // weights are at most 2^(kShift + kGrow) = 2^14
 constexpr long long kBudget = 4000000000LL;  // cycles, about 2 s
 constexpr int kPanel = 128 * 128;   // bytes of 64 columns of 128 rows
 constexpr uint32_t kTmemCols = 512; // S of both streams, then O of both: 128 columns each
 
-template <int D, bool PAIR>
+template <int D, bool E4M3, bool PAIR>
 struct Smem {
     static constexpr int kTile = D / 64 * kPanel;
-    static constexpr int kStages = PAIR ? 2 : 3;  // of K, and of V
+    static constexpr int kStages = PAIR || E4M3 ? 2 : 3;         // of K, and of V
+    static constexpr int kRaw = E4M3 ? (PAIR ? 2 : 4) : 0;       // raw tiles on their way
     static constexpr int kQ = 0;
     static constexpr int kK = (PAIR ? 2 : 1) * kTile;
     static constexpr int kV = kK + kStages * kTile;
-    static constexpr int kBar = kV + kStages * kTile;
+    static constexpr int kRing = kV + kStages * kTile;
+    static constexpr int kExps = kRing + kRaw * kTile / 2;       // [4 tiles][128 keys][2] bytes
+    static constexpr int kBar = kExps + (E4M3 ? 4 * kKeyTile * 2 : 0);
     static constexpr int kMask = kBar + 256;
     static constexpr int kBytes = kMask + kMaxTiles;
+    static_assert(kBytes <= 232448, "shared memory of a CTA");
 };
 
 __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr, uint32_t panel_bytes) {
@@ -96,6 +103,46 @@ __device__ __forceinline__ void tmem_st_wait() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// 64 consecutive columns of this thread's TMEM lane. The load and its wait are one statement, so no use
+// of the values can move above the wait.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float* v) {
+    uint32_t r[64];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63"
+        "}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+          "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+          "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+          "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+          "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]),
+          "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+          "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+          "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Registers a thread of this warpgroup: the sum over the block's is what it was launched with.
+template <int N>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// The softmax warps' own barrier.
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
 // fp16 2^e for e <= 0, twice.
@@ -111,7 +158,7 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
 
 template <int D, bool E4M3, bool PAIR>
 __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedArgs a) {
-    using L = Smem<D, PAIR>;
+    using L = Smem<D, E4M3, PAIR>;
     constexpr int STAGES = L::kStages;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::kBar);
@@ -135,20 +182,86 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
     const int split = blockIdx.x, h = blockIdx.y;
     const int row_base = blockIdx.z * (PAIR ? 2 : 1) * kRowTile;
     const int all_tiles = (a.prefix_len + kKeyTile - 1) / kKeyTile;
-    const int cta_splits = gridDim.x;
-    const int tile0 = static_cast<int>(static_cast<long long>(all_tiles) * split / cta_splits);
-    const int n_tiles = static_cast<int>(static_cast<long long>(all_tiles) * (split + 1) / cta_splits) - tile0;
+    const int tile0 = static_cast<int>(static_cast<long long>(all_tiles) * split / gridDim.x);
+    const int n_tiles = static_cast<int>(static_cast<long long>(all_tiles) * (split + 1) / gridDim.x) - tile0;
     const int all_pages = (a.prefix_len + kPageTokens - 1) / kPageTokens;
+    const size_t part = (static_cast<size_t>(split) * a.n_kv + h) * a.prefix_rows;
 
     if ((smem_u32(sm) & 1023) != 0 || n_tiles > kMaxTiles) {
         // Not reached: the operands need a 1024-byte aligned base, the list of pages its length.
+        const float bad = __int_as_float(0x7fc00000);
         for (int r = tid; r < (PAIR ? 2 : 1) * kRowTile && row_base + r < rows; r += kPrefixThreads) {
-            const size_t part = PAIR ? split : split * 2;
-            const float bad = __int_as_float(0x7fc00000);
-            a.prefix_ml[(part * a.n_kv + h) * a.prefix_rows + row_base + r] = make_float2(bad, bad);
+            a.prefix_ml[part + row_base + r] = make_float2(bad, bad);
         }
         return;
     }
+
+    // ---------------------------------------------------------------- loaders: tiles on their way
+    // Loader warp w brings the 32 keys of pages 2w, 2w + 1 of each tile; operations are K 0, V 0, K 1, ...
+    constexpr int ROW = E4M3 ? D : 2 * D;                // bytes of a pool row
+    constexpr int CHUNKS = ROW / 16;                     // 16-byte pieces of a row
+    constexpr int LOADS = CHUNKS;                        // pieces of 32 rows, a lane
+    const int lw = warp & 3;
+    int ids = -1;  // lane: page 2w + (lane & 1) of tile (lane / 2) of the 16 looked up
+    auto issue = [&](int n, uint8_t* to) {  // in order
+        const int j = n >> 1, kind = n & 1;
+        if (!kind && (j & 15) == 0) {
+            const int t = j + lane / 2;
+            const int logical = (tile0 + t) * kPagesPerTile + 2 * lw + (lane & 1);
+            ids = t < n_tiles && logical < all_pages ? __ldg(a.prefix_table + logical) : -1;
+        }
+        const uint8_t* base = static_cast<const uint8_t*>(kind ? a.v : a.k);
+        const int left = a.prefix_len - (tile0 + j) * kKeyTile - lw * 32;  // keys of this warp's 32 that exist
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int page = __shfl_sync(0xffffffffu, ids, (j & 15) * 2 + half);
+            const bool in = page >= 0 && page < a.n_pages;
+            const size_t row0 = (static_cast<size_t>(in ? page : 0) * a.n_kv + h) * kPageTokens;
+            const uint8_t* from = base + row0 * ROW;
+#pragma unroll
+            for (int i = 0; i < LOADS / 2; ++i) {
+                const int x = i * 32 + lane, r = x / CHUNKS, c = x % CHUNKS, key = lw * 32 + half * 16 + r;
+                uint8_t* dst = E4M3 ? to + key * D + c * 16
+                                    : to + (c >> 3) * kPanel + key * 128 + (((c & 7) ^ (key & 7)) * 16);
+                // A key that is not there becomes zeros.
+                const int bytes = in && half * 16 + r < left ? 16 : 0;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)),
+                             "l"(from + x * 16), "r"(bytes)
+                             : "memory");
+            }
+            if (E4M3 && !kind && lane < 8) {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                                 smem_u32(sm + L::kExps + ((j & 3) * kKeyTile + lw * 32 + half * 16) * 2 + lane * 4)),
+                             "l"(a.exps + row0 * 2 + lane * 4), "r"(in ? 4 : 0)
+                             : "memory");
+            }
+        }
+    };
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    auto raw = [&](int n) { return sm + L::kRing + n % (L::kRaw ? L::kRaw : 1) * (L::kTile / 2); };
+    const int ops = 2 * n_tiles;
+    const bool is_loader = warp >= 8 && warp < 12;
+    if (E4M3 && is_loader) {
+#pragma unroll
+        for (int n = 0; n < L::kRaw - 1; ++n) {
+            if (n < ops) issue(n, raw(n));
+            commit();
+        }
+    }
+    // ---------------------------------------------------------------- softmax: this thread's row of Q
+    const int s = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
+    const int row = row_base + (PAIR ? s * kRowTile : 0) + r;
+    const bool live = warp < 8 && row < rows;
+    uint4 q[D / 8];
+    if (warp < 8) {
+        const uint16_t* p = static_cast<const uint16_t*>(a.q) +
+                            (live ? row / a.group * a.q_stride + (h * a.group + row % a.group) * D : 0);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            q[i] = live ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+        }
+    }
+
     if (tid == 0) {
         mbar_init(q_full, PAIR ? 8 : 4);
         for (int i = 0; i < STAGES; ++i) {
@@ -173,25 +286,25 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
     // The CTA's good pages and the largest bytes of its keys.
     for (int p = tid; p < n_tiles * kPagesPerTile; p += kPrefixThreads) {
         const int logical = tile0 * kPagesPerTile + p;
-        const int page = logical < all_pages ? a.prefix_table[logical] : -1;
+        const int page = logical < all_pages ? __ldg(a.prefix_table + logical) : -1;
         if (page < 0 || page >= a.n_pages) continue;
         atomicOr(reinterpret_cast<unsigned*>(mask) + p / 32, 1u << (p % 32));
         if constexpr (E4M3) {
-            const uint4* e = reinterpret_cast<const uint4*>(
+            const uint32_t* e = reinterpret_cast<const uint32_t*>(
                 a.exps + (static_cast<size_t>(page) * a.n_kv + h) * kPageTokens * 2);
-            const uint32_t* e4 = reinterpret_cast<const uint32_t*>(e);
             const int n = min(kPageTokens, a.prefix_len - logical * kPageTokens);
-            uint32_t kt = 0, vt = 0;
+            uint32_t w[kPageTokens / 2], kt = 0, vt = 0;
+#pragma unroll
+            for (int i = 0; i < kPageTokens / 2; ++i) w[i] = __ldg(e + i);
 #pragma unroll
             for (int i = 0; i < kPageTokens / 2; ++i) {
-                const uint32_t x = __ldg(e4 + i);
                 if (2 * i < n) {
-                    kt = max(kt, x & 0xffu);
-                    vt = max(vt, x >> 8 & 0xffu);
+                    kt = max(kt, w[i] & 0xffu);
+                    vt = max(vt, w[i] >> 8 & 0xffu);
                 }
                 if (2 * i + 1 < n) {
-                    kt = max(kt, x >> 16 & 0xffu);
-                    vt = max(vt, x >> 24);
+                    kt = max(kt, w[i] >> 16 & 0xffu);
+                    vt = max(vt, w[i] >> 24);
                 }
             }
             atomicMax(&top_s[0], static_cast<int>(kt));
@@ -206,8 +319,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
     // Steps of a stream: its key tiles.
     auto steps_of = [&](int s) { return PAIR ? n_tiles : (n_tiles + 1 - s) / 2; };
 
-    if (warp == 12) {
-        if (lane == 0) {
+    if (warp >= 12) {
+        fewer_registers<kFewRegs>();
+        if (warp == 12 && lane == 0) {
             // ------------------------------------------------------------ issuer
             const uint32_t idesc_s = E4M3 ? idesc_f16_f32(kRowTile, kKeyTile) : idesc_bf16_f32(kRowTile, kKeyTile);
             const uint32_t idesc_pv = (E4M3 ? idesc_f16_f32(kRowTile, D) : idesc_bf16_f32(kRowTile, D)) |
@@ -245,13 +359,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
 #pragma unroll
                     for (int kk = 0; kk < kKeyTile / 16; ++kk) {
                         const uint64_t v = desc_mn_sw128(v_addr + kk * 16 * 128, kPanel);
-                        if constexpr (E4M3) {
-                            mma_a_tmem(o, p + kk * 8, v, idesc_pv, i > 0 || kk > 0);
-                        } else {
-                            const uint32_t at = p + (kk >> 1) * 32 + (kk & 1) * 8;
-                            mma_a_tmem(o, at, v, idesc_pv, i > 0 || kk > 0);
-                            mma_a_tmem(o, at + 16, v, idesc_pv, 1);
-                        }
+                        mma_a_tmem(o, p + kk * 8, v, idesc_pv, i > 0 || kk > 0);
+                        if constexpr (!E4M3) mma_a_tmem(o, p + 64 + kk * 8, v, idesc_pv, 1);
                     }
                     if (!PAIR || s == 1) mma_commit(&v_empty[st]);
                     if (i + 1 < steps_of(s)) ok = scores(s, i + 1);
@@ -267,132 +376,120 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
             }
         }
         __syncwarp();
-    } else if (warp >= 8) {
+    } else if (is_loader) {
         // ---------------------------------------------------------------- loaders
-        constexpr int ROW = E4M3 ? D : 2 * D;      // bytes of a pool row
-        constexpr int CHUNKS = ROW / 16;           // 16-byte pieces of a row
-        constexpr int LANES = 128 / CHUNKS;        // rows that one round of loads covers
-        constexpr int LOADS = kKeyTile / LANES;    // rounds of a tile
-        constexpr int BATCH = LOADS < 8 ? LOADS : 8;
-        constexpr int BATCHES = LOADS / BATCH;     // of a tile
-        const int lt = tid - 256, c = lt % CHUNKS, r0 = lt / CHUNKS;
-        const int total = n_tiles * 2 * BATCHES;   // K 0, V 0, K 1, V 1, ...
-        uint4 raw[2][BATCH];
-        uint32_t ex[2][BATCH];
-        auto load = [&](int n, uint4 (&x)[BATCH], uint32_t (&e)[BATCH]) {
-            const int j = n / (2 * BATCHES), kind = n / BATCHES & 1, part = n % BATCHES;
-            const uint8_t* base = static_cast<const uint8_t*>(kind ? a.v : a.k);
+        fewer_registers<kFewRegs>();
+        bool ok = true;
+        if constexpr (E4M3) {
+            for (int n = 0; ok && n < ops; ++n) {
+                const int j = n >> 1, kind = n & 1, st = j % STAGES;
+                asm volatile("cp.async.wait_group %0;" ::"n"(L::kRaw - 2) : "memory");
+                __syncwarp();
+                if (n + L::kRaw - 1 < ops) issue(n + L::kRaw - 1, raw(n + L::kRaw - 1));
+                commit();
+                if (!mbar_wait_warp(kind ? &v_empty[st] : &k_empty[st], ((j / STAGES) & 1) ^ 1, kBudget, abort)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t* to = sm + (kind ? L::kV : L::kK) + st * L::kTile;
+                const uint8_t* exps = sm + L::kExps + (j & 3) * kKeyTile * 2 + kind;
+                const int top = kind ? top_v : top_k;
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                const int r = r0 + (part * BATCH + i) * LANES;
-                const int key = (tile0 + j) * kKeyTile + r;
-                x[i] = make_uint4(0, 0, 0, 0);
-                e[i] = 0;
-                if (key >= a.prefix_len) continue;
-                const int page = __ldg(a.prefix_table + key / kPageTokens);
-                if (page < 0 || page >= a.n_pages) continue;
-                const size_t row = (static_cast<size_t>(page) * a.n_kv + h) * kPageTokens + key % kPageTokens;
-                x[i] = *reinterpret_cast<const uint4*>(base + row * ROW + c * 16);
-                if constexpr (E4M3) e[i] = a.exps[row * 2 + kind];
-            }
-        };
-        auto store = [&](int n, const uint4 (&x)[BATCH], const uint32_t (&e)[BATCH]) {
-            const int j = n / (2 * BATCHES), kind = n / BATCHES & 1, part = n % BATCHES;
-            const int st = j % STAGES;
-            uint8_t* to = sm + (kind ? L::kV : L::kK) + st * L::kTile;
-            if (part == 0 && !mbar_wait_warp(kind ? &v_empty[st] : &k_empty[st], ((j / STAGES) & 1) ^ 1,
-                                             kBudget, abort)) {
-                return false;
-            }
-#pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                const int r = r0 + (part * BATCH + i) * LANES;
-                if constexpr (E4M3) {
-                    const uint32_t f = half2_pow2(static_cast<int>(e[i]) - (kind ? top_v : top_k));
-                    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                for (int i = 0; i < LOADS; ++i) {
+                    const int x = i * 32 + lane, key = lw * 32 + x / CHUNKS, c = x % CHUNKS;
+                    const uint4 codes = *reinterpret_cast<const uint4*>(raw(n) + key * D + c * 16);
+                    const uint32_t f = half2_pow2(min(static_cast<int>(exps[key * 2]) - top, 0));
+                    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
                     uint32_t y[8];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        y[2 * q] = mul_half2(e4m3x2_to_f16x2(w[q]), f);
-                        y[2 * q + 1] = mul_half2(e4m3x2_hi_to_f16x2(w[q]), f);
+                    for (int k = 0; k < 4; ++k) {
+                        y[2 * k] = mul_half2(e4m3x2_to_f16x2(w[k]), f);
+                        y[2 * k + 1] = mul_half2(e4m3x2_hi_to_f16x2(w[k]), f);
                     }
-                    uint8_t* row = to + (c >> 2) * kPanel + r * 128;
+                    uint8_t* line = to + (c >> 2) * kPanel + key * 128;
                     const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
                     // The pieces of one row go to different banks: the second panel's halves swapped.
                     const int first = (c >> 2) & 1;
-                    *reinterpret_cast<uint4*>(row + ((((c & 3) * 2 + first) ^ (r & 7)) * 16)) = first ? hi : lo;
-                    *reinterpret_cast<uint4*>(row + ((((c & 3) * 2 + 1 - first) ^ (r & 7)) * 16)) = first ? lo : hi;
-                } else {
-                    *reinterpret_cast<uint4*>(to + (c >> 3) * kPanel + r * 128 + (((c & 7) ^ (r & 7)) * 16)) = x[i];
+                    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2 + first) ^ (key & 7)) * 16)) = first ? hi : lo;
+                    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2 + 1 - first) ^ (key & 7)) * 16)) = first ? lo : hi;
                 }
-            }
-            if (part == BATCHES - 1) {
                 fence_smem_to_mma();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(kind ? &v_full[st] : &k_full[st]);
             }
-            return true;
-        };
-        load(0, raw[0], ex[0]);
-        bool ok = true;
-        for (int n = 0; ok && n < total; n += 2) {  // total is even
-            load(n + 1, raw[1], ex[1]);
-            ok = store(n, raw[0], ex[0]);
-            if (ok && n + 2 < total) load(n + 2, raw[0], ex[0]);
-            ok = ok && store(n + 1, raw[1], ex[1]);
-        }
-        if (!ok) *abort = 1;
-    } else {
-        // ---------------------------------------------------------------- softmax
-        const int s = warp >> 2, r = (warp & 3) * 32 + lane;
-        const int row = row_base + (PAIR ? s * kRowTile : 0) + r;
-        const bool live = row < rows;
-        float c = 1.4426950408889634f / sqrtf(static_cast<float>(D));
-        {
-            // This row of Q into the operand, scaled by a power of two for fp16.
-            const uint16_t* q = static_cast<const uint16_t*>(a.q) +
-                                (live ? row / a.group * a.q_stride + (h * a.group + row % a.group) * D : 0);
-            uint4 x[D / 8];
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                x[i] = live ? reinterpret_cast<const uint4*>(q)[i] : make_uint4(0, 0, 0, 0);
-            }
-            if constexpr (E4M3) {
-                uint32_t* w = reinterpret_cast<uint32_t*>(x);
-                float big = 0.0f;
-#pragma unroll
-                for (int i = 0; i < D / 2; ++i) {
-                    big = max3(big, fabsf(a.f16 ? f16_lo(w[i]) : bf16_lo(w[i])),
-                               fabsf(a.f16 ? f16_hi(w[i]) : bf16_hi(w[i])));
-                }
-                int e = 0;
-                if (big > 0.0f && big < INFINITY) {
-                    e = min(13 + 127 - static_cast<int>(__float_as_uint(big) >> 23), 126);
-                }
-                const float f = pow2(e);
-#pragma unroll
-                for (int i = 0; i < D / 2; ++i) {
-                    w[i] = pack2_out((a.f16 ? f16_lo(w[i]) : bf16_lo(w[i])) * f,
-                                     (a.f16 ? f16_hi(w[i]) : bf16_hi(w[i])) * f, 1);
-                }
-                // Kept a normal number: a masked score is -infinity times it.
-                c = fminf(fmaxf(c * pow2(-e) * exp_of_byte(static_cast<uint32_t>(top_k)), 1e-37f), 1e37f);
-            }
-            if (PAIR || s == 0) {
-                uint8_t* to = sm + L::kQ + (PAIR ? s * L::kTile : 0) + r * 128;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    *reinterpret_cast<uint4*>(to + (i >> 3) * kPanel + (((i & 7) ^ (r & 7)) * 16)) = x[i];
-                }
+        } else {
+            // Operation n - 1 is handed over once n is on its way, or at once if n has to wait for room.
+            auto hand_over = [&](int n) {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
                 fence_smem_to_mma();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(q_full);
+                if (lane == 0) mbar_arrive(n & 1 ? &v_full[(n >> 1) % STAGES] : &k_full[(n >> 1) % STAGES]);
+            };
+            int handed = 0;
+            for (int n = 0; ok && n < ops; ++n) {
+                const int j = n >> 1, kind = n & 1, st = j % STAGES;
+                uint64_t* empty = kind ? &v_empty[st] : &k_empty[st];
+                const uint32_t parity = ((j / STAGES) & 1) ^ 1;
+                if (!__all_sync(0xffffffffu, mbar_test_wait(empty, parity))) {
+                    for (; handed < n; ++handed) hand_over(handed);
+                    ok = mbar_wait_warp(empty, parity, kBudget, abort);
+                    if (!ok) break;
+                }
+                issue(n, sm + (kind ? L::kV : L::kK) + st * L::kTile);
+                commit();
+                if (handed < n) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    fence_smem_to_mma();
+                    __syncwarp();
+                    for (; handed < n; ++handed) {
+                        if (lane == 0) mbar_arrive(handed & 1 ? &v_full[(handed >> 1) % STAGES] : &k_full[(handed >> 1) % STAGES]);
+                    }
+                }
             }
+            for (; ok && handed < ops; ++handed) hand_over(handed);
+        }
+        if (!ok) *abort = 1;
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else {
+        // ---------------------------------------------------------------- softmax
+        more_registers<kManyRegs>();
+        float c = 1.4426950408889634f / sqrtf(static_cast<float>(D));
+        if constexpr (E4M3) {
+            // The row scaled by a power of two for fp16.
+            uint32_t* w = reinterpret_cast<uint32_t*>(q);
+            float big = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 2; ++i) {
+                big = max3(big, fabsf(a.f16 ? f16_lo(w[i]) : bf16_lo(w[i])),
+                           fabsf(a.f16 ? f16_hi(w[i]) : bf16_hi(w[i])));
+            }
+            int e = 0;
+            if (big > 0.0f && big < INFINITY) {
+                e = min(13 + 127 - static_cast<int>(__float_as_uint(big) >> 23), 126);
+            }
+            const float f = pow2(e);
+#pragma unroll
+            for (int i = 0; i < D / 2; ++i) {
+                w[i] = pack2_out((a.f16 ? f16_lo(w[i]) : bf16_lo(w[i])) * f,
+                                 (a.f16 ? f16_hi(w[i]) : bf16_hi(w[i])) * f, 1);
+            }
+            // Kept a normal number: a masked score is -infinity times it.
+            c = fminf(fmaxf(c * pow2(-e) * exp_of_byte(static_cast<uint32_t>(top_k)), 1e-37f), 1e37f);
+        }
+        if (PAIR || s == 0) {
+            uint8_t* to = sm + L::kQ + (PAIR ? s * L::kTile : 0) + r * 128;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                *reinterpret_cast<uint4*>(to + (i >> 3) * kPanel + (((i & 7) ^ (r & 7)) * 16)) = q[i];
+            }
+            fence_smem_to_mma();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
         }
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + s * 128, o_at = tmem + lanes + 256 + s * 128;
         float m = -INFINITY, neg = kShift;
-        float2 l2 = make_float2(0.0f, 0.0f);
+        float2 l4[4] = {};
         const int steps = steps_of(s);
         bool ok = true;
         for (int i = 0; i < steps; ++i) {
@@ -402,107 +499,143 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                 break;
             }
             tc_fence_after();
-            const bool full = mask[j] == 0xff && (tile0 + j + 1) * kKeyTile <= a.prefix_len;
-            // A key that is not there: its bit, and its place before the end.
-            auto there = [&](int k) {
-                return (mask[j] >> (k / kPageTokens) & 1) && (tile0 + j) * kKeyTile + k < a.prefix_len;
-            };
-            float top = -INFINITY;
+            float x[kKeyTile];
+            tmem_ld64(s_at, x);
+            tmem_ld64(s_at + 64, x + 64);
+            if (mask[j] != 0xff || (tile0 + j + 1) * kKeyTile > a.prefix_len) {
+                // Keys that are not there: their page's bit, their place before the end.
+                const unsigned pages = mask[j];
+                const int left = a.prefix_len - (tile0 + j) * kKeyTile;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float x[32];
-                tmem_ld32(s_at + q * 32, x);
-                if (!full) {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) x[k] = there(q * 32 + k) ? x[k] : -INFINITY;
+                for (int k = 0; k < kKeyTile; ++k) {
+                    if (!(pages >> (k / kPageTokens) & 1) || k >= left) x[k] = -INFINITY;
                 }
-#pragma unroll
-                for (int k = 0; k < 32; k += 2) top = max3(top, x[k], x[k + 1]);
             }
-            if (__any_sync(0xffffffffu, top * c > m + kGrow)) {
-                const float m_new = fmaxf(m, top * c);
+            float top4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+            for (int k = 4; k < kKeyTile; k += 8) {
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    if (k + z + 4 < kKeyTile) top4[z] = max3(top4[z], x[k + z], x[k + z + 4]);
+                    else top4[z] = fmaxf(top4[z], x[k + z]);
+                }
+            }
+            const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * c;
+            if (__any_sync(0xffffffffu, top > m + kGrow)) {
+                const float m_new = fmaxf(m, top);
                 const float f = m_new == m ? 1.0f : ex2(m - m_new);
                 m = m_new;
                 neg = kShift - (m_new == -INFINITY ? 0.0f : m_new);
-                l2.x *= f;
-                l2.y *= f;
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    l4[z].x *= f;
+                    l4[z].y *= f;
+                }
                 if (i > 0) {  // the products before this tile's scores are done: O is still
 #pragma unroll 1
-                    for (int q = 0; q < D / 32; ++q) {
-                        float x[32];
-                        uint32_t y[32];
-                        tmem_ld32(o_at + q * 32, x);
+                    for (int k = 0; k < D / 32; ++k) {
+                        float y[32];
+                        uint32_t z[32];
+                        tmem_ld32(o_at + k * 32, y);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) y[k] = __float_as_uint(x[k] * f);
-                        tmem_st32(o_at + q * 32, y);
+                        for (int e = 0; e < 32; ++e) z[e] = __float_as_uint(y[e] * f);
+                        tmem_st32(o_at + k * 32, z);
                     }
-                    tmem_st_wait();
                 }
             }
             const float2 c2 = make_float2(c, c), n2 = make_float2(neg, neg);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                uint32_t y[32];  // fp16: 64 keys; bf16: 32 keys at a time, hi and lo
+                uint32_t y[32];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const int k0 = (half * 2 + q) * 32;
-                    float x[32];
-                    tmem_ld32(s_at + k0, x);
-                    if (!full) {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) x[k] = there(k0 + k) ? x[k] : -INFINITY;
+                for (int k = 0; k < 64; k += 2) {
+                    float2 p = ffma2(make_float2(x[half * 64 + k], x[half * 64 + k + 1]), c2, n2);
+                    p.x = ex2(p.x);
+                    p.y = ex2(p.y);
+                    l4[(k >> 1) & 3] = fadd2(l4[(k >> 1) & 3], p);
+                    if constexpr (E4M3) {
+                        y[k / 2] = pack2_out(p.x, p.y, 1);
+                    } else {
+                        y[k / 2] = pack2_bf16(p.x, p.y);
+                        x[half * 64 + k] = p.x - bf16_lo(y[k / 2]);
+                        x[half * 64 + k + 1] = p.y - bf16_hi(y[k / 2]);
                     }
-#pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        float2 p = ffma2(make_float2(x[k], x[k + 1]), c2, n2);
-                        p.x = ex2(p.x);
-                        p.y = ex2(p.y);
-                        l2 = fadd2(l2, p);
-                        if constexpr (E4M3) {
-                            y[q * 16 + k / 2] = pack2_out(p.x, p.y, 1);
-                        } else {
-                            const uint32_t w = pack2_bf16(p.x, p.y);
-                            y[k / 2] = w;
-                            y[16 + k / 2] = pack2_bf16(p.x - bf16_lo(w), p.y - bf16_hi(w));
-                        }
-                    }
-                    if constexpr (!E4M3) tmem_st32(s_at + k0, y);
                 }
-                if constexpr (E4M3) tmem_st32(s_at + half * 32, y);
+                tmem_st32(s_at + half * 32, y);
+                if constexpr (!E4M3) {
+#pragma unroll
+                    for (int k = 0; k < 64; k += 2) y[k / 2] = pack2_bf16(x[half * 64 + k], x[half * 64 + k + 1]);
+                    tmem_st32(s_at + 64 + half * 32, y);
+                }
             }
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[s]);
         }
-        if (ok && steps > 0) ok = mbar_wait_warp(&o_full[s], 0, kBudget, abort);
+        // All products are done, of both streams: the operands' room takes the sums, so that they leave as
+        // whole rows (16 KB a warp for D = 128; the 16-byte pieces swizzled by their row).
+        for (int z = 0; z < 2; ++z) {
+            if (ok && steps_of(z) > 0) ok = mbar_wait_warp(&o_full[z], 0, kBudget, abort);
+        }
         if (!ok) *abort = 1;
-        const size_t part = PAIR ? split : split * 2 + s;
-        const size_t at = (part * a.n_kv + h) * a.prefix_rows + row;
-        const float f_v = E4M3 ? exp_of_byte(static_cast<uint32_t>(top_v)) : 1.0f;
         tc_fence_after();
+        float l = ((l4[0].x + l4[0].y) + (l4[1].x + l4[1].y)) + ((l4[2].x + l4[2].y) + (l4[3].x + l4[3].y));
+        float f = E4M3 ? exp_of_byte(static_cast<uint32_t>(top_v)) : 1.0f;
+        if constexpr (!PAIR) {
+            // Both streams' rows relative to the larger of their maxima.
+            float2* ml_s = reinterpret_cast<float2*>(sm + L::kQ);
+            ml_s[s * kRowTile + r] = make_float2(m, l);
+            softmax_sync();
+            const float2 other = ml_s[(s ^ 1) * kRowTile + r];
+            const float both = fmaxf(m, other.x);
+            const float mine = m == both ? 1.0f : ex2(m - both), theirs = other.x == both ? 1.0f : ex2(other.x - both);
+            l = l * mine + other.y * theirs;
+            f *= mine;
+            m = both;
+        }
+        constexpr int PIECES = D / 4;  // 16-byte pieces of a row of sums
+        float4* mine_s = reinterpret_cast<float4*>(sm + L::kK) + warp * 32 * PIECES;
 #pragma unroll 1
-        for (int q = 0; q < D / 32; ++q) {
-            float x[32];
+        for (int k = 0; k < D / 32; ++k) {
+            float y[32];
             if (ok && steps > 0) {
-                tmem_ld32(o_at + q * 32, x);
+                tmem_ld32(o_at + k * 32, y);
             } else {
 #pragma unroll
-                for (int k = 0; k < 32; ++k) x[k] = 0.0f;
+                for (int e = 0; e < 32; ++e) y[e] = 0.0f;
             }
-            if (live) {
-                float4* to = reinterpret_cast<float4*>(a.prefix_o + at * D + q * 32);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    to[k] = make_float4(x[4 * k] * f_v, x[4 * k + 1] * f_v, x[4 * k + 2] * f_v, x[4 * k + 3] * f_v);
-                }
+            for (int e = 0; e < 8; ++e) {
+                mine_s[lane * PIECES + ((k * 8 + e) ^ (lane & (PIECES - 1)))] =
+                    make_float4(y[4 * e] * f, y[4 * e + 1] * f, y[4 * e + 2] * f, y[4 * e + 3] * f);
             }
-        }
-        if (live) {
-            const float bad = __int_as_float(0x7fc00000);
-            a.prefix_ml[at] = ok ? make_float2(m, l2.x + l2.y) : make_float2(bad, bad);
         }
         tc_fence_before();
+        if (live && (PAIR || s == 0)) {
+            const float bad = __int_as_float(0x7fc00000);
+            a.prefix_ml[part + row] = ok ? make_float2(m, l) : make_float2(bad, bad);
+        }
+        // The rows this warp writes: its own (PAIR), half of those that both streams have (SOLO).
+        constexpr int PER = 32 / PIECES < 1 ? 1 : 32 / PIECES;  // rows at once
+        if constexpr (PAIR) __syncwarp();
+        else softmax_sync();
+        const int first = PAIR ? 0 : s * 16, n_rows = PAIR ? 32 : 16;
+        const float4* one = reinterpret_cast<const float4*>(sm + L::kK) + (PAIR ? warp : warp & 3) * 32 * PIECES;
+        const float4* two = one + 4 * 32 * PIECES;
+        const int row0 = row_base + (PAIR ? s * kRowTile : 0) + (warp & 3) * 32;
+#pragma unroll 4
+        for (int i = 0; i < n_rows; i += PER) {
+            const int rr = first + i + lane / PIECES, at = rr * PIECES + (lane % PIECES ^ (rr & (PIECES - 1)));
+            float4 y = one[at];
+            if constexpr (!PAIR) {
+                const float4 z = two[at];
+                y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+            }
+            if (row0 + rr < rows) {
+                reinterpret_cast<float4*>(a.prefix_o + (part + row0 + rr) * D)[lane % PIECES] = y;
+            }
+        }
     }
     __syncthreads();
     if (warp == 12) {
@@ -514,8 +647,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
 template <int D, bool E4M3, bool PAIR>
 void launch(const PagedArgs& a, cudaStream_t s) {
     const int rows = a.n_q * a.group, tile = (PAIR ? 2 : 1) * kRowTile;
-    const dim3 grid(PAIR ? a.prefix_splits : a.prefix_splits / 2, a.n_kv, (rows + tile - 1) / tile);
-    constexpr int bytes = Smem<D, PAIR>::kBytes;
+    const dim3 grid(a.prefix_splits, a.n_kv, (rows + tile - 1) / tile);
+    constexpr int bytes = Smem<D, E4M3, PAIR>::kBytes;
     Q3_CUDA(cudaFuncSetAttribute(prefix_kernel<D, E4M3, PAIR>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     launch_dep(false, prefix_kernel<D, E4M3, PAIR>, grid, dim3(kPrefixThreads), bytes, s, a);
@@ -531,7 +664,7 @@ void launch(const PagedArgs& a, bool e4m3, cudaStream_t s) {
 }  // namespace
 
 // Parts per row. A CTA's time is about (its key tiles + 3), 3 for its start and end; the splits make the
-// sum over the waves of 148 CTAs least. PAIR CTAs leave one part, SOLO ones two.
+// sum over the waves of 148 CTAs least.
 int prefix_splits(int n_kv, int rows, int prefix_len) {
     if (prefix_len <= 0 || rows <= 0) return 0;
     const bool pair = rows > kRowTile;
@@ -547,7 +680,7 @@ int prefix_splits(int n_kv, int rows, int prefix_len) {
             best_cost = cost;
         }
     }
-    return static_cast<int>(pair ? best : 2 * best);
+    return static_cast<int>(best);
 }
 
 void launch_prefix_attention(const PagedArgs& a, int head_dim, bool e4m3, cudaStream_t s) {
