@@ -49,15 +49,17 @@ constexpr uint32_t kTmemCols = 512; // S of both streams, then O of both: 128 co
 template <int D, bool E4M3, bool PAIR>
 struct Smem {
     static constexpr int kTile = D / 64 * kPanel;
-    static constexpr int kStages = PAIR || E4M3 ? 2 : 3;         // of K, and of V
-    static constexpr int kRaw = E4M3 ? (PAIR ? 2 : 4) : 0;       // raw tiles on their way
+    static constexpr int kSlots = E4M3 ? (PAIR ? 3 : 4) : (PAIR ? 5 : 6);  // K and V tiles, in turn
+    static constexpr int kRaw = E4M3 ? 4 : 0;                              // raw tiles on their way
     static constexpr int kQ = 0;
-    static constexpr int kK = (PAIR ? 2 : 1) * kTile;
-    static constexpr int kV = kK + kStages * kTile;
-    static constexpr int kRing = kV + kStages * kTile;
-    static constexpr int kExps = kRing + kRaw * kTile / 2;       // [4 tiles][128 keys][2] bytes
-    static constexpr int kBar = kExps + (E4M3 ? 4 * kKeyTile * 2 : 0);
+    static constexpr int kKv = (PAIR ? 2 : 1) * kTile;
+    static constexpr int kRing = kKv + kSlots * kTile;
+    static constexpr int kExps = kRing + kRaw * kTile / 2;  // [4 tiles][128 keys][2] bytes
+    static constexpr int kScale = kExps + (E4M3 ? 4 * kKeyTile * 2 : 0);  // [4 warps][32 keys] fp16 pairs
+    static constexpr int kBar = kScale + (E4M3 ? kKeyTile * 4 : 0);
     static constexpr int kMask = kBar + 256;
+    // After the last product the sums of the 8 softmax warps take the tiles' room.
+    static_assert(kBar - kKv >= 8 * 32 * D * 4, "room for the sums");
     static constexpr int kBytes = kMask + kMaxTiles;
     static_assert(kBytes <= 232448, "shared memory of a CTA");
 };
@@ -159,14 +161,12 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
 template <int D, bool E4M3, bool PAIR>
 __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedArgs a) {
     using L = Smem<D, E4M3, PAIR>;
-    constexpr int STAGES = L::kStages;
+    constexpr int SLOTS = L::kSlots;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::kBar);
     uint64_t* q_full = bars;
-    uint64_t* k_full = bars + 1;
-    uint64_t* k_empty = bars + 4;
-    uint64_t* v_full = bars + 7;
-    uint64_t* v_empty = bars + 10;
+    uint64_t* full = bars + 1;    // [SLOTS]
+    uint64_t* empty = bars + 7;   // [SLOTS]
     uint64_t* s_full = bars + 13;
     uint64_t* p_full = bars + 15;
     uint64_t* o_full = bars + 17;
@@ -201,6 +201,21 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
     constexpr int ROW = E4M3 ? D : 2 * D;                // bytes of a pool row
     constexpr int CHUNKS = ROW / 16;                     // 16-byte pieces of a row
     constexpr int LOADS = CHUNKS;                        // pieces of 32 rows, a lane
+    // Lane's place in load i: for e4m3 eight rows of four pieces (of one operand panel), so that the
+    // converted pieces of two neighbouring rows fall into all banks; else rows one after the other.
+    constexpr int PANELS = E4M3 ? D / 64 : 1;
+    auto place = [&](int i, int& r, int& c) {
+        if constexpr (E4M3) {
+            r = i / PANELS * 8 + lane / 4;
+            c = i % PANELS * 4 + lane % 4;
+        } else {
+            const int x = i * 32 + lane;
+            r = x / CHUNKS;
+            c = x % CHUNKS;
+        }
+    };
+    // Its place in a raw tile: odd rows' panels swapped, so that two rows' reads fall into all banks.
+    auto raw_at = [&](int key, int c) { return key * D + (PANELS == 2 ? c ^ (key & 1) * 4 : c) * 16; };
     const int lw = warp & 3;
     int ids = -1;  // lane: page 2w + (lane & 1) of tile (lane / 2) of the 16 looked up
     auto issue = [&](int n, uint8_t* to) {  // in order
@@ -220,13 +235,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
             const uint8_t* from = base + row0 * ROW;
 #pragma unroll
             for (int i = 0; i < LOADS / 2; ++i) {
-                const int x = i * 32 + lane, r = x / CHUNKS, c = x % CHUNKS, key = lw * 32 + half * 16 + r;
-                uint8_t* dst = E4M3 ? to + key * D + c * 16
+                int rr, c;
+                place(half * (LOADS / 2) + i, rr, c);
+                const int key = lw * 32 + rr;
+                uint8_t* dst = E4M3 ? to + raw_at(key, c)
                                     : to + (c >> 3) * kPanel + key * 128 + (((c & 7) ^ (key & 7)) * 16);
                 // A key that is not there becomes zeros.
-                const int bytes = in && half * 16 + r < left ? 16 : 0;
+                const int bytes = in && rr < left ? 16 : 0;
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)),
-                             "l"(from + x * 16), "r"(bytes)
+                             "l"(from + (rr - half * 16) * ROW + c * 16), "r"(bytes)
                              : "memory");
             }
             if (E4M3 && !kind && lane < 8) {
@@ -262,34 +279,20 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
         }
     }
 
-    if (tid == 0) {
-        mbar_init(q_full, PAIR ? 8 : 4);
-        for (int i = 0; i < STAGES; ++i) {
-            mbar_init(&k_full[i], 4);
-            mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], 4);
-            mbar_init(&v_empty[i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
-            mbar_init(&o_full[i], 1);
-        }
-        mbar_init(done, 1);
-        *abort = 0;
-        top_s[0] = top_s[1] = 0;
-        mbar_fence_init();
-    }
-    for (int i = tid; i < n_tiles; i += kPrefixThreads) mask[i] = 0;
-    if (warp == 12) tmem_alloc(tmem_slot, kTmemCols);
-    __syncthreads();
-    // The CTA's good pages and the largest bytes of its keys.
-    for (int p = tid; p < n_tiles * kPagesPerTile; p += kPrefixThreads) {
+    // The CTA's pages and the largest bytes of their keys: a thread a page, the first of its pages looked
+    // up before the barriers are ready.
+    const int n_pages = min(n_tiles * kPagesPerTile, all_pages - tile0 * kPagesPerTile);
+    struct Look {
+        bool in;
+        int k, v;
+    };
+    auto look_up = [&](int p) {
+        Look x{false, 0, 0};
+        if (p >= n_pages) return x;
         const int logical = tile0 * kPagesPerTile + p;
-        const int page = logical < all_pages ? __ldg(a.prefix_table + logical) : -1;
-        if (page < 0 || page >= a.n_pages) continue;
-        atomicOr(reinterpret_cast<unsigned*>(mask) + p / 32, 1u << (p % 32));
-        if constexpr (E4M3) {
+        const int page = __ldg(a.prefix_table + logical);
+        x.in = page >= 0 && page < a.n_pages;
+        if (E4M3 && x.in) {
             const uint32_t* e = reinterpret_cast<const uint32_t*>(
                 a.exps + (static_cast<size_t>(page) * a.n_kv + h) * kPageTokens * 2);
             const int n = min(kPageTokens, a.prefix_len - logical * kPageTokens);
@@ -307,8 +310,39 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                     vt = max(vt, w[i] >> 24);
                 }
             }
-            atomicMax(&top_s[0], static_cast<int>(kt));
-            atomicMax(&top_s[1], static_cast<int>(vt));
+            x.k = static_cast<int>(kt);
+            x.v = static_cast<int>(vt);
+        }
+        return x;
+    };
+    Look mine = look_up(tid);
+
+    if (tid == 0) {
+        mbar_init(q_full, PAIR ? 8 : 4);
+        for (int i = 0; i < SLOTS; ++i) {
+            mbar_init(&full[i], 4);
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_full[i], 1);
+        }
+        mbar_init(done, 1);
+        *abort = 0;
+        top_s[0] = top_s[1] = 0;
+        mbar_fence_init();
+    }
+    for (int i = tid; i < n_tiles; i += kPrefixThreads) mask[i] = 0;
+    if (warp == 12) tmem_alloc(tmem_slot, kTmemCols);
+    __syncthreads();
+    for (int p = tid; p < n_pages; p += kPrefixThreads) {
+        if (p != tid) mine = look_up(p);
+        if (!mine.in) continue;
+        atomicOr(reinterpret_cast<unsigned*>(mask) + p / 32, 1u << (p % 32));
+        if constexpr (E4M3) {
+            atomicMax(&top_s[0], mine.k);
+            atomicMax(&top_s[1], mine.v);
         }
     }
     tc_fence_before();
@@ -328,18 +362,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                                       (1u << 16);  // B MN-major
             bool ok = mbar_wait(q_full, 0, kBudget, abort);
             auto scores = [&](int s, int i) {
-                const int j = PAIR ? i : 2 * i + s, st = j % STAGES;
-                if (!mbar_wait(&k_full[st], (j / STAGES) & 1, kBudget, abort)) return false;
+                const int n = 2 * (PAIR ? i : 2 * i + s), slot = n % SLOTS;
+                if (!mbar_wait(&full[slot], (n / SLOTS) & 1, kBudget, abort)) return false;
                 tc_fence_after();
                 const uint32_t q_addr = smem_u32(sm + L::kQ + (PAIR ? s * L::kTile : 0));
-                const uint32_t k_addr = smem_u32(sm + L::kK + st * L::kTile);
+                const uint32_t k_addr = smem_u32(sm + L::kKv + slot * L::kTile);
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
                     mma_bf16(tmem + s * 128, desc_k_sw128(q_addr + (kk >> 2) * kPanel) + 2 * (kk & 3),
                              desc_k_sw128(k_addr + (kk >> 2) * kPanel) + 2 * (kk & 3), idesc_s, kk > 0);
                 }
                 mma_commit(&s_full[s]);
-                if (!PAIR || s == 1) mma_commit(&k_empty[st]);
+                if (!PAIR || s == 1) mma_commit(&empty[slot]);
                 return true;
             };
             for (int s = 0; s < 2 && ok; ++s) {
@@ -349,12 +383,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
             for (int i = 0; ok && i < most; ++i) {
                 for (int s = 0; s < 2 && ok; ++s) {
                     if (i >= steps_of(s)) continue;
-                    const int j = PAIR ? i : 2 * i + s, st = j % STAGES;
+                    const int n = 2 * (PAIR ? i : 2 * i + s) + 1, slot = n % SLOTS;
                     ok = mbar_wait(&p_full[s], i & 1, kBudget, abort) &&
-                         mbar_wait(&v_full[st], (j / STAGES) & 1, kBudget, abort);
+                         mbar_wait(&full[slot], (n / SLOTS) & 1, kBudget, abort);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t v_addr = smem_u32(sm + L::kV + st * L::kTile);
+                    const uint32_t v_addr = smem_u32(sm + L::kKv + slot * L::kTile);
                     const uint32_t o = tmem + 256 + s * 128, p = tmem + s * 128;
 #pragma unroll
                     for (int kk = 0; kk < kKeyTile / 16; ++kk) {
@@ -362,7 +396,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                         mma_a_tmem(o, p + kk * 8, v, idesc_pv, i > 0 || kk > 0);
                         if constexpr (!E4M3) mma_a_tmem(o, p + 64 + kk * 8, v, idesc_pv, 1);
                     }
-                    if (!PAIR || s == 1) mma_commit(&v_empty[st]);
+                    if (!PAIR || s == 1) mma_commit(&empty[slot]);
                     if (i + 1 < steps_of(s)) ok = scores(s, i + 1);
                     else mma_commit(&o_full[s]);
                 }
@@ -381,41 +415,41 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
         fewer_registers<kFewRegs>();
         bool ok = true;
         if constexpr (E4M3) {
+            uint32_t* scale = reinterpret_cast<uint32_t*>(sm + L::kScale) + lw * 32;
             for (int n = 0; ok && n < ops; ++n) {
-                const int j = n >> 1, kind = n & 1, st = j % STAGES;
+                const int j = n >> 1, kind = n & 1, slot = n % SLOTS;
                 asm volatile("cp.async.wait_group %0;" ::"n"(L::kRaw - 2) : "memory");
                 __syncwarp();
+                // A lane a key: its power of two relative to the largest.
+                const int e = sm[L::kExps + ((j & 3) * kKeyTile + lw * 32 + lane) * 2 + kind];
+                scale[lane] = half2_pow2(min(e - (kind ? top_v : top_k), 0));
                 if (n + L::kRaw - 1 < ops) issue(n + L::kRaw - 1, raw(n + L::kRaw - 1));
                 commit();
-                if (!mbar_wait_warp(kind ? &v_empty[st] : &k_empty[st], ((j / STAGES) & 1) ^ 1, kBudget, abort)) {
+                if (!mbar_wait_warp(&empty[slot], ((n / SLOTS) & 1) ^ 1, kBudget, abort)) {
                     ok = false;
                     break;
                 }
-                uint8_t* to = sm + (kind ? L::kV : L::kK) + st * L::kTile;
-                const uint8_t* exps = sm + L::kExps + (j & 3) * kKeyTile * 2 + kind;
-                const int top = kind ? top_v : top_k;
+                __syncwarp();
+                uint8_t* to = sm + L::kKv + slot * L::kTile;
+                const uint8_t* from = raw(n);
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i) {
-                    const int x = i * 32 + lane, key = lw * 32 + x / CHUNKS, c = x % CHUNKS;
-                    const uint4 codes = *reinterpret_cast<const uint4*>(raw(n) + key * D + c * 16);
-                    const uint32_t f = half2_pow2(min(static_cast<int>(exps[key * 2]) - top, 0));
-                    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-                    uint32_t y[8];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        y[2 * k] = mul_half2(e4m3x2_to_f16x2(w[k]), f);
-                        y[2 * k + 1] = mul_half2(e4m3x2_hi_to_f16x2(w[k]), f);
-                    }
+                    int rr, c;
+                    place(i, rr, c);
+                    const int key = lw * 32 + rr;
+                    const uint4 w = *reinterpret_cast<const uint4*>(from + raw_at(key, c));
+                    const uint32_t f = scale[rr];
                     uint8_t* line = to + (c >> 2) * kPanel + key * 128;
-                    const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
-                    // The pieces of one row go to different banks: the second panel's halves swapped.
-                    const int first = (c >> 2) & 1;
-                    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2 + first) ^ (key & 7)) * 16)) = first ? hi : lo;
-                    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2 + 1 - first) ^ (key & 7)) * 16)) = first ? lo : hi;
+                    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2) ^ (key & 7)) * 16)) =
+                        make_uint4(mul_half2(e4m3x2_to_f16x2(w.x), f), mul_half2(e4m3x2_hi_to_f16x2(w.x), f),
+                                   mul_half2(e4m3x2_to_f16x2(w.y), f), mul_half2(e4m3x2_hi_to_f16x2(w.y), f));
+                    *reinterpret_cast<uint4*>(line + ((((c & 3) * 2 + 1) ^ (key & 7)) * 16)) =
+                        make_uint4(mul_half2(e4m3x2_to_f16x2(w.z), f), mul_half2(e4m3x2_hi_to_f16x2(w.z), f),
+                                   mul_half2(e4m3x2_to_f16x2(w.w), f), mul_half2(e4m3x2_hi_to_f16x2(w.w), f));
                 }
                 fence_smem_to_mma();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(kind ? &v_full[st] : &k_full[st]);
+                if (lane == 0) mbar_arrive(&full[slot]);
             }
         } else {
             // Operation n - 1 is handed over once n is on its way, or at once if n has to wait for room.
@@ -423,26 +457,25 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
                 fence_smem_to_mma();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(n & 1 ? &v_full[(n >> 1) % STAGES] : &k_full[(n >> 1) % STAGES]);
+                if (lane == 0) mbar_arrive(&full[n % SLOTS]);
             };
             int handed = 0;
             for (int n = 0; ok && n < ops; ++n) {
-                const int j = n >> 1, kind = n & 1, st = j % STAGES;
-                uint64_t* empty = kind ? &v_empty[st] : &k_empty[st];
-                const uint32_t parity = ((j / STAGES) & 1) ^ 1;
-                if (!__all_sync(0xffffffffu, mbar_test_wait(empty, parity))) {
+                const int slot = n % SLOTS;
+                const uint32_t parity = ((n / SLOTS) & 1) ^ 1;
+                if (!__all_sync(0xffffffffu, mbar_test_wait(&empty[slot], parity))) {
                     for (; handed < n; ++handed) hand_over(handed);
-                    ok = mbar_wait_warp(empty, parity, kBudget, abort);
+                    ok = mbar_wait_warp(&empty[slot], parity, kBudget, abort);
                     if (!ok) break;
                 }
-                issue(n, sm + (kind ? L::kV : L::kK) + st * L::kTile);
+                issue(n, sm + L::kKv + slot * L::kTile);
                 commit();
                 if (handed < n) {
                     asm volatile("cp.async.wait_group 1;" ::: "memory");
                     fence_smem_to_mma();
                     __syncwarp();
                     for (; handed < n; ++handed) {
-                        if (lane == 0) mbar_arrive(handed & 1 ? &v_full[(handed >> 1) % STAGES] : &k_full[(handed >> 1) % STAGES]);
+                        if (lane == 0) mbar_arrive(&full[handed % SLOTS]);
                     }
                 }
             }
@@ -595,7 +628,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
             m = both;
         }
         constexpr int PIECES = D / 4;  // 16-byte pieces of a row of sums
-        float4* mine_s = reinterpret_cast<float4*>(sm + L::kK) + warp * 32 * PIECES;
+        float4* mine_s = reinterpret_cast<float4*>(sm + L::kKv) + warp * 32 * PIECES;
 #pragma unroll 1
         for (int k = 0; k < D / 32; ++k) {
             float y[32];
@@ -621,7 +654,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
         if constexpr (PAIR) __syncwarp();
         else softmax_sync();
         const int first = PAIR ? 0 : s * 16, n_rows = PAIR ? 32 : 16;
-        const float4* one = reinterpret_cast<const float4*>(sm + L::kK) + (PAIR ? warp : warp & 3) * 32 * PIECES;
+        const float4* one = reinterpret_cast<const float4*>(sm + L::kKv) + (PAIR ? warp : warp & 3) * 32 * PIECES;
         const float4* two = one + 4 * 32 * PIECES;
         const int row0 = row_base + (PAIR ? s * kRowTile : 0) + (warp & 3) * 32;
 #pragma unroll 4
