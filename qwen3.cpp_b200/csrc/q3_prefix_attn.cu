@@ -77,14 +77,37 @@ __device__ __forceinline__ void fence_smem_to_mma() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
+
+// The tensor-core instructions of the issuing thread, which is chosen by elect.sync. (Issued by lane 0 of
+// an ordinary branch an MMA takes about 95 cycles to issue, more than its 64 in the pipe.)
+// D[tmem] (+)= A[smem] * B[smem]^T
+__device__ __forceinline__ void issue_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // D[tmem] (+)= A[tmem] * B[smem]: A's rows are TMEM lanes, two 16-bit values a column.
-__device__ __forceinline__ void mma_a_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                           uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void issue_mma_a_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                                 uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
         "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void issue_commit(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
         : "memory");
 }
 
@@ -146,6 +169,18 @@ __device__ __forceinline__ void fewer_registers() {
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+// The same, NaN if one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
 // fp16 2^e for e <= 0, twice.
 __device__ __forceinline__ uint32_t half2_pow2(int e) {
@@ -168,10 +203,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
     uint64_t* full = bars + 1;    // [SLOTS]
     uint64_t* empty = bars + 7;   // [SLOTS]
     uint64_t* s_full = bars + 13;
-    uint64_t* p_full = bars + 15;
-    uint64_t* o_full = bars + 17;
-    uint64_t* done = bars + 19;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+    uint64_t* p_full = bars + 15;  // [stream][half of the keys]
+    uint64_t* o_full = bars + 19;
+    uint64_t* done = bars + 21;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* top_s = reinterpret_cast<int*>(tmem_slot + 2);  // largest byte of K, of V
     uint8_t* mask = sm + L::kMask;                       // a bit a good page of each key tile
@@ -325,7 +360,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[2 * i], 4);
+            mbar_init(&p_full[2 * i + 1], 4);
             mbar_init(&o_full[i], 1);
         }
         mbar_init(done, 1);
@@ -348,32 +384,35 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const int top_k = top_s[0], top_v = top_s[1];
     // Steps of a stream: its key tiles.
     auto steps_of = [&](int s) { return PAIR ? n_tiles : (n_tiles + 1 - s) / 2; };
 
     if (warp >= 12) {
         fewer_registers<kFewRegs>();
-        if (warp == 12 && lane == 0) {
+        if (warp == 12 && elect_one()) {
             // ------------------------------------------------------------ issuer
             const uint32_t idesc_s = E4M3 ? idesc_f16_f32(kRowTile, kKeyTile) : idesc_bf16_f32(kRowTile, kKeyTile);
             const uint32_t idesc_pv = (E4M3 ? idesc_f16_f32(kRowTile, D) : idesc_bf16_f32(kRowTile, D)) |
                                       (1u << 16);  // B MN-major
-            bool ok = mbar_wait(q_full, 0, kBudget, abort);
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                return mbar_wait(bar, parity, kBudget, abort);
+            };
+            bool ok = wait(q_full, 0);
             auto scores = [&](int s, int i) {
                 const int n = 2 * (PAIR ? i : 2 * i + s), slot = n % SLOTS;
-                if (!mbar_wait(&full[slot], (n / SLOTS) & 1, kBudget, abort)) return false;
+                if (!wait(&full[slot], (n / SLOTS) & 1)) return false;
                 tc_fence_after();
-                const uint32_t q_addr = smem_u32(sm + L::kQ + (PAIR ? s * L::kTile : 0));
-                const uint32_t k_addr = smem_u32(sm + L::kKv + slot * L::kTile);
+                const uint64_t qd = desc_k_sw128(smem_u32(sm + L::kQ + (PAIR ? s * L::kTile : 0)));
+                const uint64_t kd = desc_k_sw128(smem_u32(sm + L::kKv + slot * L::kTile));
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk) {
-                    mma_bf16(tmem + s * 128, desc_k_sw128(q_addr + (kk >> 2) * kPanel) + 2 * (kk & 3),
-                             desc_k_sw128(k_addr + (kk >> 2) * kPanel) + 2 * (kk & 3), idesc_s, kk > 0);
+                    const uint64_t at = ((kk >> 2) * kPanel >> 4) + 2 * (kk & 3);
+                    issue_mma(tmem + s * 128, qd + at, kd + at, idesc_s, kk > 0);
                 }
-                mma_commit(&s_full[s]);
-                if (!PAIR || s == 1) mma_commit(&empty[slot]);
+                issue_commit(&s_full[s]);
+                if (!PAIR || s == 1) issue_commit(&empty[slot]);
                 return true;
             };
             for (int s = 0; s < 2 && ok; ++s) {
@@ -381,30 +420,36 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
             }
             const int most = steps_of(0);
             for (int i = 0; ok && i < most; ++i) {
-                for (int s = 0; s < 2 && ok; ++s) {
-                    if (i >= steps_of(s)) continue;
-                    const int n = 2 * (PAIR ? i : 2 * i + s) + 1, slot = n % SLOTS;
-                    ok = mbar_wait(&p_full[s], i & 1, kBudget, abort) &&
-                         mbar_wait(&full[slot], (n / SLOTS) & 1, kBudget, abort);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t v_addr = smem_u32(sm + L::kKv + slot * L::kTile);
-                    const uint32_t o = tmem + 256 + s * 128, p = tmem + s * 128;
 #pragma unroll
-                    for (int kk = 0; kk < kKeyTile / 16; ++kk) {
-                        const uint64_t v = desc_mn_sw128(v_addr + kk * 16 * 128, kPanel);
-                        mma_a_tmem(o, p + kk * 8, v, idesc_pv, i > 0 || kk > 0);
-                        if constexpr (!E4M3) mma_a_tmem(o, p + 64 + kk * 8, v, idesc_pv, 1);
-                    }
-                    if (!PAIR || s == 1) mma_commit(&empty[slot]);
+                for (int s = 0; s < 2; ++s) {
+                    if (!ok || i >= steps_of(s)) continue;
+                    const int n = 2 * (PAIR ? i : 2 * i + s) + 1, slot = n % SLOTS;
+                    ok = wait(&full[slot], (n / SLOTS) & 1) && wait(&p_full[2 * s], i & 1);
+                    if (!ok) continue;
+                    tc_fence_after();
+                    const uint64_t vd = desc_mn_sw128(smem_u32(sm + L::kKv + slot * L::kTile), kPanel);
+                    const uint32_t o = tmem + 256 + s * 128, p = tmem + s * 128;
+                    auto product = [&](int kk) {
+                        const uint64_t v = vd + kk * (16 * 128 >> 4);
+                        issue_mma_a_tmem(o, p + kk * 8, v, idesc_pv, i > 0 || kk > 0);
+                        if constexpr (!E4M3) issue_mma_a_tmem(o, p + 64 + kk * 8, v, idesc_pv, 1);
+                    };
+#pragma unroll
+                    for (int kk = 0; kk < kKeyTile / 32; ++kk) product(kk);
+                    ok = wait(&p_full[2 * s + 1], i & 1);
+                    if (!ok) continue;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = kKeyTile / 32; kk < kKeyTile / 16; ++kk) product(kk);
+                    if (!PAIR || s == 1) issue_commit(&empty[slot]);
                     if (i + 1 < steps_of(s)) ok = scores(s, i + 1);
-                    else mma_commit(&o_full[s]);
+                    else issue_commit(&o_full[s]);
                 }
             }
             if (!ok) *abort = 1;
             // Nothing is in flight when the CTA ends.
-            mma_commit(done);
-            if (!mbar_wait(done, 0, kBudget, abort)) {
+            issue_commit(done);
+            if (!wait(done, 0)) {
                 const long long t0 = clock64();
                 while (!mbar_try_wait(done, 0) && clock64() - t0 < kBudget) {}
             }
@@ -432,20 +477,28 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                 __syncwarp();
                 uint8_t* to = sm + L::kKv + slot * L::kTile;
                 const uint8_t* from = raw(n);
+                // All reads first: the compiler does not move one above a write.
+                uint4 w[LOADS];
+                uint32_t f[LOADS];
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    int rr, c;
+                    place(i, rr, c);
+                    w[i] = *reinterpret_cast<const uint4*>(from + raw_at(lw * 32 + rr, c));
+                    f[i] = scale[rr];
+                }
 #pragma unroll
                 for (int i = 0; i < LOADS; ++i) {
                     int rr, c;
                     place(i, rr, c);
                     const int key = lw * 32 + rr;
-                    const uint4 w = *reinterpret_cast<const uint4*>(from + raw_at(key, c));
-                    const uint32_t f = scale[rr];
                     uint8_t* line = to + (c >> 2) * kPanel + key * 128;
                     *reinterpret_cast<uint4*>(line + ((((c & 3) * 2) ^ (key & 7)) * 16)) =
-                        make_uint4(mul_half2(e4m3x2_to_f16x2(w.x), f), mul_half2(e4m3x2_hi_to_f16x2(w.x), f),
-                                   mul_half2(e4m3x2_to_f16x2(w.y), f), mul_half2(e4m3x2_hi_to_f16x2(w.y), f));
+                        make_uint4(mul_half2(e4m3x2_to_f16x2(w[i].x), f[i]), mul_half2(e4m3x2_hi_to_f16x2(w[i].x), f[i]),
+                                   mul_half2(e4m3x2_to_f16x2(w[i].y), f[i]), mul_half2(e4m3x2_hi_to_f16x2(w[i].y), f[i]));
                     *reinterpret_cast<uint4*>(line + ((((c & 3) * 2 + 1) ^ (key & 7)) * 16)) =
-                        make_uint4(mul_half2(e4m3x2_to_f16x2(w.z), f), mul_half2(e4m3x2_hi_to_f16x2(w.z), f),
-                                   mul_half2(e4m3x2_to_f16x2(w.w), f), mul_half2(e4m3x2_hi_to_f16x2(w.w), f));
+                        make_uint4(mul_half2(e4m3x2_to_f16x2(w[i].z), f[i]), mul_half2(e4m3x2_hi_to_f16x2(w[i].z), f[i]),
+                                   mul_half2(e4m3x2_to_f16x2(w[i].w), f[i]), mul_half2(e4m3x2_hi_to_f16x2(w[i].w), f[i]));
                 }
                 fence_smem_to_mma();
                 __syncwarp();
@@ -549,16 +602,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
             for (int k = 4; k < kKeyTile; k += 8) {
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
-                    if (k + z + 4 < kKeyTile) top4[z] = max3(top4[z], x[k + z], x[k + z + 4]);
-                    else top4[z] = fmaxf(top4[z], x[k + z]);
+                    if (k + z + 4 < kKeyTile) top4[z] = max3_nan(top4[z], x[k + z], x[k + z + 4]);
+                    else top4[z] = max_nan(top4[z], x[k + z]);
                 }
             }
-            const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * c;
-            if (__any_sync(0xffffffffu, top > m + kGrow)) {
-                const float m_new = fmaxf(m, top);
+            const float top = max_nan(max_nan(top4[0], top4[1]), max_nan(top4[2], top4[3])) * c;
+            if (__any_sync(0xffffffffu, !(top <= m + kGrow))) {
+                const float m_new = max_nan(m, top);
                 const float f = m_new == m ? 1.0f : ex2(m - m_new);
                 m = m_new;
-                neg = kShift - (m_new == -INFINITY ? 0.0f : m_new);
+                // A row that has seen NaN or +infinity stays NaN.
+                neg = m < INFINITY ? kShift - (m == -INFINITY ? 0.0f : m) : __int_as_float(0x7fc00000);
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
                     l4[z].x *= f;
@@ -577,6 +631,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                 }
             }
             const float2 c2 = make_float2(c, c), n2 = make_float2(neg, neg);
+            // Half the keys at a time: the product over the first half starts while the second is at work.
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 uint32_t y[32];
@@ -585,26 +640,27 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                     float2 p = ffma2(make_float2(x[half * 64 + k], x[half * 64 + k + 1]), c2, n2);
                     p.x = ex2(p.x);
                     p.y = ex2(p.y);
-                    l4[(k >> 1) & 3] = fadd2(l4[(k >> 1) & 3], p);
-                    if constexpr (E4M3) {
-                        y[k / 2] = pack2_out(p.x, p.y, 1);
-                    } else {
-                        y[k / 2] = pack2_bf16(p.x, p.y);
-                        x[half * 64 + k] = p.x - bf16_lo(y[k / 2]);
-                        x[half * 64 + k + 1] = p.y - bf16_hi(y[k / 2]);
-                    }
+                    x[half * 64 + k] = p.x;
+                    x[half * 64 + k + 1] = p.y;
+                    y[k / 2] = E4M3 ? pack2_out(p.x, p.y, 1) : pack2_bf16(p.x, p.y);
                 }
                 tmem_st32(s_at + half * 32, y);
                 if constexpr (!E4M3) {
+                    uint32_t lo[32];
 #pragma unroll
-                    for (int k = 0; k < 64; k += 2) y[k / 2] = pack2_bf16(x[half * 64 + k], x[half * 64 + k + 1]);
-                    tmem_st32(s_at + 64 + half * 32, y);
+                    for (int k = 0; k < 64; k += 2) {
+                        lo[k / 2] = pack2_bf16(x[half * 64 + k] - bf16_lo(y[k / 2]), x[half * 64 + k + 1] - bf16_hi(y[k / 2]));
+                    }
+                    tmem_st32(s_at + 64 + half * 32, lo);
                 }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[2 * s + half]);
             }
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[s]);
+            // The sum of the weights, while the products run.
+#pragma unroll
+            for (int k = 0; k < kKeyTile; k += 2) l4[(k >> 1) & 3] = fadd2(l4[(k >> 1) & 3], make_float2(x[k], x[k + 1]));
         }
         // All products are done, of both streams: the operands' room takes the sums, so that they leave as
         // whole rows (16 KB a warp for D = 128; the 16-byte pieces swizzled by their row).
