@@ -42,16 +42,22 @@ namespace q3 {
 
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;                // of a block on the line, and of the join
 constexpr int kThreads = kWarps * 32;
+constexpr int kStripWarps = 8;           // of a strip's block
 constexpr float kGrow = 4.0f;  // how far (log2) a score may pass the running maximum
 constexpr int kGrowV = 3;      // the same for V's powers of two
 
-// Pages of a warp's ring, and blocks a multiprocessor (registers and rings together).
-template <bool E4M3, int NT>
+// Tables of up to so many pages take a block a strip: 1 sequence of 512 tokens STRIP1 us against 8.4 with
+// the line, whose scan and join cost about 4 us.
+constexpr int kStripPages = 64;
+
+// Warps of a block, pages of a warp's ring, and blocks a multiprocessor (registers and rings together).
+template <bool E4M3, int NT, bool LINE>
 struct Shape {
-    static constexpr int kStages = E4M3 ? 3 : 2;
-    static constexpr int kBlocks = NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2);
+    static constexpr int kWarps = LINE ? q3::kWarps : kStripWarps;
+    static constexpr int kStages = E4M3 && !LINE ? 3 : 2;
+    static constexpr int kBlocks = LINE ? (NT == 1 ? (E4M3 ? 5 : 3) : (E4M3 ? 4 : 3)) : (E4M3 ? (NT == 1 ? 2 : 1) : 1);
 };
 
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from) {
@@ -187,12 +193,12 @@ __device__ __forceinline__ int row_groups(const SeqShape& s, int group) {
 // Joins one row's n parts and writes its head, by one warp: a lane looks up a part's weight and place
 // (part_of(i, ml, o)), then all lanes add the part's sums, several parts on their way at once. The
 // order is the parts', whoever joins them.
+// It starts from a part that the warp already has: (top, its sum in lane 0 and 0 elsewhere, y).
 template <int D, typename PartOf>
-__device__ __forceinline__ void join_row(int n, PartOf part_of, uint16_t* out, int f16) {
+__device__ __forceinline__ void join_row(float top, float sum, float (&y)[D / 32], int n, PartOf part_of,
+                                         uint16_t* out, int f16) {
     constexpr int V = D / 32;
     const int lane = threadIdx.x & 31;
-    float top = -INFINITY, sum = 0.0f;  // sum: this lane's parts
-    float y[V] = {};
     for (int i0 = 0; i0 < n; i0 += 32) {
         float2 ml = make_float2(-INFINITY, 0.0f);
         const float* o = nullptr;
@@ -240,92 +246,111 @@ __device__ __forceinline__ long long run_length(long long total, unsigned blocks
     return max(static_cast<long long>(kMinUnits), (total + blocks - 1) / static_cast<long long>(blocks));
 }
 
-template <int D, bool E4M3, int NT>
+template <int D, bool E4M3, int NT, bool LINE>
 struct OwnSmem {
     static constexpr int kRow = E4M3 ? D : 2 * D;                  // bytes of a pool row
     static constexpr int kPage = 2 * kPageTokens * kRow + (E4M3 ? 2 * kPageTokens : 0);  // K, V, bytes
-    static constexpr int kRing = kWarps * Shape<E4M3, NT>::kStages * kPage;
-    static constexpr int kSums = kWarps * 8 * NT * D * 4;          // after a run of pages, in its place
+    static constexpr int kRing = Shape<E4M3, NT, LINE>::kWarps * Shape<E4M3, NT, LINE>::kStages * kPage;
+    static constexpr int kSums = Shape<E4M3, NT, LINE>::kWarps * 8 * NT * D * 4;          // after a run of pages, in its place
     static constexpr int kBytes = kRing > kSums ? kRing : kSums;
 };
 
-template <int D, bool E4M3, int NT>
-__global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
+// LINE: the block takes its run of the line of units. Else it takes one strip and finishes its rows, the
+// prefix's parts among them.
+template <int D, bool E4M3, int NT, bool LINE>
+__global__ void __launch_bounds__(Shape<E4M3, NT, LINE>::kWarps * 32, Shape<E4M3, NT, LINE>::kBlocks)
     own_pages_kernel(const PagedArgs a) {
     constexpr int MT = D / 16;                    // m-tiles of O^T, k-steps of S^T
-    constexpr int KW = E4M3 ? D / 16 : D / 8;     // words a lane holds of one K row
     constexpr int VW = E4M3 ? D / 32 : D / 16;    // and of one V row
-    using L = OwnSmem<D, E4M3, NT>;
-    constexpr int ROW = L::kRow, PIECES = ROW / 16, STAGES = Shape<E4M3, NT>::kStages;
+    using L = OwnSmem<D, E4M3, NT, LINE>;
+    constexpr int W = Shape<E4M3, NT, LINE>::kWarps;
+    constexpr int ROW = L::kRow, PIECES = ROW / 16, STAGES = Shape<E4M3, NT, LINE>::kStages;
     constexpr int ROWS = 8 * NT;
     extern __shared__ __align__(128) uint8_t ring_s[];
     float (*o_s)[ROWS][D] = reinterpret_cast<float (*)[ROWS][D]>(ring_s);
-    __shared__ float m_s[kWarps][ROWS], l_s[kWarps][ROWS];
-    __shared__ long long scan_s[kWarps];
+    __shared__ float m_s[W][ROWS], l_s[W][ROWS];
+    __shared__ long long scan_s[W];
     __shared__ long long first_s;
     __shared__ int seq_s;
 
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
 
-    // This block's run of units.
-    const int per_thread = (a.n_seqs + kThreads - 1) / kThreads;
-    const int b0 = min(tid * per_thread, a.n_seqs), b1 = min(b0 + per_thread, a.n_seqs);
-    auto units = [&](int b) { return seq_units<NT>(a, seq_shape(a, b)); };
-    long long mine = 0, before, total;
-    for (int b = b0; b < b1; ++b) mine += units(b);
-    block_scan(mine, scan_s, before, total);
-    const long long per = run_length(total, gridDim.x);
-    const long long start = per * blockIdx.x, end = min(total, start + per);
-    if (start >= end) {
-        pdl_wait();
-        return;
-    }
-    if (before <= start && start < before + mine) {
-        long long x = before;
-        int b = b0;
-        for (long long u; x + (u = units(b)) <= start; ++b) x += u;
-        seq_s = b;
-        first_s = x;
-    }
-    __syncthreads();
-
     const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(ring_s)) + warp * STAGES * L::kPage;
     const float scale = 1.4426950408889634f / sqrtf(static_cast<float>(D));
-    long long pos = start, seq_first = first_s;
-    int b = seq_s;
+    long long pos = 0, end = 1, seq_first = 0;
+    int b, h, rg, ids = -1;
+    if constexpr (LINE) {
+        // This block's run of units.
+        const int per_thread = (a.n_seqs + W * 32 - 1) / W * 32;
+        const int b0 = min(tid * per_thread, a.n_seqs), b1 = min(b0 + per_thread, a.n_seqs);
+        auto units = [&](int i) { return seq_units<NT>(a, seq_shape(a, i)); };
+        long long mine = 0, before, total;
+        for (int i = b0; i < b1; ++i) mine += units(i);
+        block_scan(mine, scan_s, before, total);
+        const long long per = run_length(total, gridDim.x);
+        pos = per * blockIdx.x;
+        end = min(total, pos + per);
+        if (pos >= end) {
+            pdl_wait();
+            return;
+        }
+        if (before <= pos && pos < before + mine) {
+            long long x = before;
+            int i = b0;
+            for (long long u; x + (u = units(i)) <= pos; ++i) x += u;
+            seq_s = i;
+            first_s = x;
+        }
+        __syncthreads();
+        seq_first = first_s;
+        b = seq_s;
+    } else {
+        const unsigned most = (a.max_q * a.group + ROWS - 1) / ROWS;
+        rg = static_cast<int>(blockIdx.x % most);
+        h = static_cast<int>(blockIdx.x / most % a.n_kv);
+        b = static_cast<int>(blockIdx.x / most / a.n_kv);
+        // The first pages' numbers are on their way with the lengths.
+        const int p = warp + lane * W;
+        if (p < a.table_stride) ids = a.table[static_cast<size_t>(b) * a.table_stride + p];
+    }
     while (pos < end) {
         const SeqShape s = seq_shape(a, b);
         const int pages = seq_pages(s), groups = row_groups<NT>(s, a.group);
-        const int each = strip_units(pages);
-        const long long all = static_cast<long long>(a.n_kv) * groups * each;
-        if (pos >= seq_first + all) {
-            seq_first += all;
-            ++b;
-            continue;
+        int p0 = 0, p1 = pages;
+        if constexpr (LINE) {
+            const int each = strip_units(pages);
+            const long long all = static_cast<long long>(a.n_kv) * groups * each;
+            if (pos >= seq_first + all) {
+                seq_first += all;
+                ++b;
+                continue;
+            }
+            const long long strip = (pos - seq_first) / each;  // (head, row group)
+            const long long strip_first = seq_first + strip * each;
+            const long long u1 = min(strip_first + each, end);
+            // This block's pages of it: all of them, or the run's beginning or end cuts them.
+            p0 = static_cast<int>(max(0LL, pos - strip_first - kSetup));
+            p1 = min(pages, static_cast<int>(u1 - strip_first) - kSetup);
+            pos = u1;
+            if (u1 - strip_first <= kSetup) continue;  // the run ends in front of the strip's first page
+            h = static_cast<int>(strip / groups);
+            rg = static_cast<int>(strip % groups);
+        } else {
+            pos = end;
+            if (rg >= groups) break;
         }
-        const long long strip = (pos - seq_first) / each;  // (head, row group)
-        const long long strip_first = seq_first + strip * each;
-        const long long u1 = min(strip_first + each, end);
-        // This block's pages of it: all of them, or the run's beginning or end cuts them.
-        const int p0 = static_cast<int>(max(0LL, pos - strip_first - kSetup));
-        const int p1 = min(pages, static_cast<int>(u1 - strip_first) - kSetup);
-        const bool touched = u1 - strip_first > kSetup;
-        pos = u1;
-        if (!touched) continue;  // the run ends in front of the strip's first page
-        const int h = static_cast<int>(strip / groups), rg = static_cast<int>(strip % groups);
         const int r_base = rg * ROWS;
         const int n_rows = min(ROWS, s.rows * a.group - r_base);
 
         // This warp's pages, the first of them on their way.
         const int32_t* table = a.table + static_cast<size_t>(b) * a.table_stride;
-        const int steps = p1 - p0 > warp ? (p1 - p0 - warp + kWarps - 1) / kWarps : 0;
-        int ids = 0;
+        const int steps = p1 - p0 > warp ? (p1 - p0 - warp + W - 1) / W : 0;
         uint32_t fill = ring, page_s = ring;  // the ring's next page to fill, to use
         unsigned good = 0;  // of the last 32 steps looked up: whether the page is in the pool
         auto start_page = [&](int it) {  // in order: 0, 1, 2, ...
-            if ((it & 31) == 0) {
-                const int p = p0 + warp + (it + lane) * kWarps;
+            if ((it & 31) == 0 && (LINE || it > 0)) {
+                const int p = p0 + warp + (it + lane) * W;
                 ids = p < p1 ? table[p] : -1;
             }
             const int page = __shfl_sync(0xffffffffu, ids, it & 31);
@@ -356,8 +381,8 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
 
         // Q as the B operand: lane (g, t) holds row g's values in the order of K's.
         uint32_t qw[NT][D / 8];
-        float c_col[NT][2];  // score factor of the columns 2t, 2t + 1
-        int seen[NT][2];     // keys that they see
+        float c_col[E4M3 ? NT : 1][2];  // score factor of the columns 2t, 2t + 1 (a bf16 pool has one for all)
+        c_col[0][0] = scale;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int r = r_base + n * 8 + g;
@@ -378,7 +403,6 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
                     w[3] = x.w;
                 }
             }
-            float c = scale;
             if constexpr (E4M3) {
                 float big = 0.0f;
 #pragma unroll
@@ -400,24 +424,20 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
                     const float hi = a.f16 ? f16_hi(qw[n][i]) : bf16_hi(qw[n][i]);
                     qw[n][i] = pack2_out(lo * f, hi * f, 1);
                 }
-                c = scale * pow2(-e);
-            }
+                const float c = scale * pow2(-e);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int rr = n * 8 + 2 * t + x;
-                c_col[n][x] = __shfl_sync(0xffffffffu, c, (2 * t + x) * 4);
-                seen[n][x] = rr < n_rows ? s.len - s.rows + (r_base + rr) / a.group + 1 : 0;
+                for (int x = 0; x < 2; ++x) c_col[n][x] = __shfl_sync(0xffffffffu, c, (2 * t + x) * 4);
             }
         }
         const int tail_key = s.len - s.rows + r_base / a.group + 1;  // seen by every row below it
 
-        float m[NT][2], lim[NT][2], neg[NT][2], l[NT][2], o[NT][MT][4];  // lim = m + kGrow, neg = kShift - m
+        float m[NT][2], neg[NT][2], l[NT][2], o[NT][MT][4];  // neg = kShift - m
         int r_v = -1000;  // power of two that o is relative to
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                m[n][x] = lim[n][x] = -INFINITY;
+                m[n][x] = -INFINITY;
                 neg[n][x] = kShift;
                 l[n][x] = 0.0f;
             }
@@ -426,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
         }
 
         for (int it = 0; it < steps; ++it) {
-            const int key0 = (p0 + warp + it * kWarps) * kPageTokens;
+            const int key0 = (p0 + warp + it * W) * kPageTokens;
             copy_wait<STAGES - 2>();
             __syncwarp();  // every lane's copies of this page are in, and its reads of the one before done
             // `good` grows a bit a page looked up: this page's is (pages looked up since) from its end.
@@ -434,32 +454,37 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
             if (it + STAGES - 1 < steps) start_page(it + STAGES - 1);
             copy_commit();
             constexpr int SW = PIECES < 8 ? PIECES - 1 : 7;
-            uint32_t kr[2][KW], vr[4][VW], ex[2] = {0, 0};
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-#pragma unroll
-                for (int j = 0; j < PIECES / 4; ++j) {
-                    lds_16(page_s + (g + 8 * x) * ROW + ((k_piece<PIECES>(t, j) ^ (g & SW)) * 16), &kr[x][4 * j]);
-                }
-            }
+            uint32_t ex[2] = {0, 0};
             if constexpr (E4M3) {
                 ex[0] = lds_u16(page_s + 2 * kPageTokens * ROW + g * 2);
                 ex[1] = lds_u16(page_s + 2 * kPageTokens * ROW + g * 2 + 16);
             }
             float sc[NT][4];
+            constexpr int PER = E4M3 ? 4 : 2;  // k-steps of a 16-byte piece
+            uint32_t kr[2][2][4];              // this piece and the next, of both keys
+            auto read_k = [&](int j) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    lds_16(page_s + (g + 8 * x) * ROW + ((k_piece<PIECES>(t, j) ^ (g & SW)) * 16), kr[j & 1][x]);
+                }
+            };
+            read_k(0);
 #pragma unroll
             for (int k = 0; k < MT; ++k) {
+                const int j = k / PER, w = k % PER;
+                if (w == 0 && j + 1 < PIECES / 4) read_k(j + 1);
+                const uint32_t (&kp)[2][4] = kr[j & 1];
                 uint32_t f[4];
                 if constexpr (E4M3) {
-                    f[0] = e4m3x2_to_f16x2(kr[0][k]);
-                    f[1] = e4m3x2_to_f16x2(kr[1][k]);
-                    f[2] = e4m3x2_hi_to_f16x2(kr[0][k]);
-                    f[3] = e4m3x2_hi_to_f16x2(kr[1][k]);
+                    f[0] = e4m3x2_to_f16x2(kp[0][w]);
+                    f[1] = e4m3x2_to_f16x2(kp[1][w]);
+                    f[2] = e4m3x2_hi_to_f16x2(kp[0][w]);
+                    f[3] = e4m3x2_hi_to_f16x2(kp[1][w]);
                 } else {
-                    f[0] = kr[0][2 * k];
-                    f[1] = kr[1][2 * k];
-                    f[2] = kr[0][2 * k + 1];
-                    f[3] = kr[1][2 * k + 1];
+                    f[0] = kp[0][2 * w];
+                    f[1] = kp[1][2 * w];
+                    f[2] = kp[0][2 * w + 1];
+                    f[3] = kp[1][2 * w + 1];
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -475,11 +500,16 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float x = sc[n][i] * c_col[n][i & 1];
+                    float x = sc[n][i] * (E4M3 ? c_col[n][i & 1] : c_col[0][0]);
                     if constexpr (E4M3) x *= __uint_as_float((ex[i >> 1] & 0xffu) << 23);  // 2^(byte - 127)
-                    if (tail && (!there || key0 + g + 8 * (i >> 1) >= seen[n][i & 1])) x = -INFINITY;
+                    if (tail) {
+                        // Keys that this column's row sees: none for a row past the last.
+                        const int rr = n * 8 + 2 * t + (i & 1);
+                        const int seen = there && rr < n_rows ? s.len - s.rows + (r_base + rr) / a.group + 1 : 0;
+                        if (key0 + g + 8 * (i >> 1) >= seen) x = -INFINITY;
+                    }
                     p[n][i] = x;
-                    grow |= x > lim[n][i & 1];
+                    grow |= x > m[n][i & 1] + kGrow;
                 }
             }
             int v_top = 0;
@@ -508,7 +538,6 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
                         const float m_new = fmaxf(m[n][x], mx);
                         f[x] = m_new == m[n][x] ? 1.0f : ex2(m[n][x] - m_new);
                         m[n][x] = m_new;
-                        lim[n][x] = m_new + kGrow;
                         neg[n][x] = kShift - (m_new == -INFINITY ? 0.0f : m_new);
                         l[n][x] *= f[x];
                         f[x] *= fv;
@@ -550,69 +579,74 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
                     }
                 }
             }
+            // O^T += V^T P^T, a 16-byte piece of the four keys at a time.
+            constexpr int VP = VW < 4 ? VW : 4;  // words of a piece
+            bool odd_any = false;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int r = 2 * t + (x & 1) + 8 * (x >> 1);
-                const uint32_t at = page_s + (kPageTokens + r) * ROW;
-                if constexpr (E4M3 && D == 64) {
-                    lds_8(at + (((g >> 1) ^ (r & SW)) * 16) + (g & 1) * 8, vr[x]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < VW / 4; ++j) lds_16(at + (((j * 8 + g) ^ (r & SW)) * 16), &vr[x][4 * j]);
-                }
-            }
-            bool odd = false;
-            if (tail) {
-                // Values of keys that are not there are anything, NaN too: as zeros they add nothing.
+            for (int j = 0; j < VW / VP; ++j) {
+                uint32_t vr[4][VP];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    const bool here = 2 * t + (x & 1) + 8 * (x >> 1) < limit;
-#pragma unroll
-                    for (int w = 0; w < VW; ++w) {
-                        vr[x][w] = here ? vr[x][w] : 0u;
-                        odd |= odd_word<E4M3>(vr[x][w]);
-                    }
+                    const int r = 2 * t + (x & 1) + 8 * (x >> 1);
+                    const uint32_t at = page_s + (kPageTokens + r) * ROW;
+                    if constexpr (VP == 2) lds_8(at + (((g >> 1) ^ (r & SW)) * 16) + (g & 1) * 8, vr[x]);
+                    else lds_16(at + (((j * 8 + g) ^ (r & SW)) * 16), vr[x]);
                 }
-            }
-            if (tail && __any_sync(0xffffffffu, odd)) {
-                // An infinity or NaN that some rows see and others do not: token by token, with the keys
-                // that the token does not see as zeros.
-                const int first = r_base / a.group, last = (r_base + n_rows - 1) / a.group;
-                for (int tok = first; tok <= last; ++tok) {
-                    const int lim = there ? s.len - s.rows + tok + 1 - key0 : 0;
-                    uint32_t vm[4][VW];
+                if (tail) {
+                    // Values of keys that are not there are anything, NaN too: as zeros they add nothing.
+                    bool odd = false;
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const bool here = 2 * t + (x & 1) + 8 * (x >> 1) < lim;
+                        const bool here = 2 * t + (x & 1) + 8 * (x >> 1) < limit;
 #pragma unroll
-                        for (int w = 0; w < VW; ++w) vm[x][w] = here ? vr[x][w] : 0u;
+                        for (int w = 0; w < VP; ++w) {
+                            vr[x][w] = here ? vr[x][w] : 0u;
+                            odd |= odd_word<E4M3>(vr[x][w]);
+                        }
                     }
+                    odd_any = __any_sync(0xffffffffu, odd);
+                }
+                constexpr int TILES = MT / (VW / VP);
+                if (tail && odd_any) {
+                    // An infinity or NaN that some rows see and others do not: token by token, with the keys
+                    // that the token does not see as zeros.
+                    const int first = r_base / a.group, last = (r_base + n_rows - 1) / a.group;
+                    for (int tok = first; tok <= last; ++tok) {
+                        const int lim = there ? s.len - s.rows + tok + 1 - key0 : 0;
+                        uint32_t vm[4][VP];
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        uint32_t f[4];
-                        v_operand<E4M3, VW>(vm, i, f);
+                        for (int x = 0; x < 4; ++x) {
+                            const bool here = 2 * t + (x & 1) + 8 * (x >> 1) < lim;
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma16816<E4M3>(c, f[0], f[1], f[2], f[3], pb[n][0], pb[n][1]);
-                            if constexpr (!E4M3) mma16816<false>(c, f[0], f[1], f[2], f[3], pl[n][0], pl[n][1]);
+                            for (int w = 0; w < VP; ++w) vm[x][w] = here ? vr[x][w] : 0u;
+                        }
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                if ((r_base + n * 8 + 2 * t + (j & 1)) / a.group == tok) o[n][i][j] += c[j];
+                        for (int i = 0; i < TILES; ++i) {
+                            uint32_t f[4];
+                            v_operand<E4M3, VP>(vm, i, f);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma16816<E4M3>(c, f[0], f[1], f[2], f[3], pb[n][0], pb[n][1]);
+                                if constexpr (!E4M3) mma16816<false>(c, f[0], f[1], f[2], f[3], pl[n][0], pl[n][1]);
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    if ((r_base + n * 8 + 2 * t + (q & 1)) / a.group == tok) o[n][j * TILES + i][q] += c[q];
+                                }
                             }
                         }
                     }
-                }
-            } else {
+                } else {
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    uint32_t f[4];
-                    v_operand<E4M3, VW>(vr, i, f);
+                    for (int i = 0; i < TILES; ++i) {
+                        uint32_t f[4];
+                        v_operand<E4M3, VP>(vr, i, f);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma16816<E4M3>(o[n][i], f[0], f[1], f[2], f[3], pb[n][0], pb[n][1]);
-                        if constexpr (!E4M3) {
-                            mma16816<false>(o[n][i], f[0], f[1], f[2], f[3], pl[n][0], pl[n][1]);
+                        for (int n = 0; n < NT; ++n) {
+                            mma16816<E4M3>(o[n][j * TILES + i], f[0], f[1], f[2], f[3], pb[n][0], pb[n][1]);
+                            if constexpr (!E4M3) {
+                                mma16816<false>(o[n][j * TILES + i], f[0], f[1], f[2], f[3], pl[n][0], pl[n][1]);
+                            }
                         }
                     }
                 }
@@ -643,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
                 const int r = n * 8 + 2 * t + x;
                 float top = m_s[0][r];
 #pragma unroll
-                for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][r]);
+                for (int w = 1; w < W; ++w) top = fmaxf(top, m_s[w][r]);
                 const float f = (m[n][x] == top ? 1.0f : ex2(m[n][x] - top)) * f_v;
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
@@ -655,17 +689,46 @@ __global__ void __launch_bounds__(kThreads, Shape<E4M3, NT>::kBlocks)
             }
         }
         __syncthreads();
+        if constexpr (!LINE) {
+            // A strip's block has its rows to itself: a warp a row, the prefix's parts behind its own.
+            pdl_wait();
+            const size_t split = static_cast<size_t>(a.n_kv) * a.prefix_rows;
+            for (int r = warp; r < n_rows; r += W) {
+                constexpr int V = D / 32;
+                float top = m_s[0][r], sum = 0.0f, y[V] = {};
+#pragma unroll
+                for (int w = 1; w < W; ++w) top = fmaxf(top, m_s[w][r]);
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    sum += l_s[w][r] * (m_s[w][r] == top ? 1.0f : ex2(m_s[w][r] - top));
+#pragma unroll
+                    for (int d = 0; d < V; ++d) y[d] += o_s[w][r][lane * V + d];
+                }
+                const int rr = r_base + r;
+                const size_t row = h * static_cast<size_t>(a.prefix_rows) + static_cast<size_t>(s.row0) * a.group + rr;
+                join_row<D>(
+                    top, lane == 0 ? sum : 0.0f, y, a.prefix_splits,
+                    [&](int i, const float2*& ml, const float*& o) {
+                        ml = a.prefix_ml + i * split + row;
+                        o = a.prefix_o + (i * split + row) * D;
+                    },
+                    static_cast<uint16_t*>(a.out) + (s.row0 + rr / a.group) * a.out_stride +
+                        (h * a.group + rr % a.group) * D,
+                    a.f16);
+            }
+            break;
+        }
         const bool whole = p0 == 0 && p1 == pages;
         const int part = p0 > 0 ? 0 : 1;
-        for (int at = tid; at < n_rows * (D / 4); at += kThreads) {
+        for (int at = tid; at < n_rows * (D / 4); at += W * 32) {
             const int r = at / (D / 4), d = at % (D / 4) * 4;
             float top = m_s[0][r];
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, m_s[w][r]);
+            for (int w = 1; w < W; ++w) top = fmaxf(top, m_s[w][r]);
             float sum = 0.0f;
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
+            for (int w = 0; w < W; ++w) {
                 sum += l_s[w][r] * (m_s[w][r] == top ? 1.0f : ex2(m_s[w][r] - top));
                 const float4 z = *reinterpret_cast<const float4*>(&o_s[w][r][d]);
                 y.x += z.x;
@@ -734,8 +797,9 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const PagedArgs a, const
     if (r >= s.rows * a.group || (own == 1 && a.prefix_len == 0)) return;  // no row; finished by its block
     const size_t row = h * static_cast<size_t>(a.prefix_rows) + static_cast<size_t>(s.row0) * a.group + r;
     const size_t split = static_cast<size_t>(a.n_kv) * a.prefix_rows;
+    float y[D / 32] = {};
     join_row<D>(
-        own + a.prefix_splits,
+        -INFINITY, 0.0f, y, own + a.prefix_splits,
         [&](int i, const float2*& ml, const float*& o) {
             if (i >= own) {
                 const size_t at = (i - own) * split + row;
@@ -757,14 +821,24 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const PagedArgs a, const
 template <int D, bool E4M3, int NT>
 void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
     const long long groups = (static_cast<long long>(a.max_q) * a.group + 8 * NT - 1) / (8 * NT);
+    const long long strips = static_cast<long long>(a.n_seqs) * a.n_kv * groups;
+    if (a.table_stride <= kStripPages) {
+        // Short sequences: a block a strip, no line to find and nothing to join after it.
+        constexpr int bytes = OwnSmem<D, E4M3, NT, false>::kBytes;
+        auto kernel = own_pages_kernel<D, E4M3, NT, false>;
+        Q3_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        launch_dep(a.prefix_len > 0, kernel, dim3(static_cast<unsigned>(strips)), dim3(kStripWarps * 32), bytes,
+                   s, a);
+        return;
+    }
     // No more blocks than the table's width could fill.
-    const long long most = (static_cast<long long>(a.n_seqs) * a.n_kv * (std::max(a.table_stride, 1) + kSetup) * groups +
-                            kMinUnits - 1) / kMinUnits;
-    const int grid = static_cast<int>(std::max(
-        1LL, std::min({most, static_cast<long long>(sms) * Shape<E4M3, NT>::kBlocks, static_cast<long long>(kMaxBlocks)})));
-    constexpr int bytes = OwnSmem<D, E4M3, NT>::kBytes;
-    Q3_CUDA(cudaFuncSetAttribute(own_pages_kernel<D, E4M3, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    launch_dep(a.prefix_len > 0, own_pages_kernel<D, E4M3, NT>, dim3(grid), dim3(kThreads), bytes, s, a);
+    const long long most = (strips * (a.table_stride + kSetup) + kMinUnits - 1) / kMinUnits;
+    const int grid = static_cast<int>(
+        std::min({most, static_cast<long long>(sms) * Shape<E4M3, NT, true>::kBlocks, static_cast<long long>(kMaxBlocks)}));
+    constexpr int bytes = OwnSmem<D, E4M3, NT, true>::kBytes;
+    auto kernel = own_pages_kernel<D, E4M3, NT, true>;
+    Q3_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    launch_dep(a.prefix_len > 0, kernel, dim3(grid), dim3(kThreads), bytes, s, a);
     const long long rows = static_cast<long long>(a.n_seqs) * a.n_kv * a.max_q * a.group;
     launch_dep(true, join_kernel<D, NT>, dim3(static_cast<unsigned>((rows + kWarps - 1) / kWarps)),
                dim3(kThreads), 0, s, a, static_cast<unsigned>(grid));
