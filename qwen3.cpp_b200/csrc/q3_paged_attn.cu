@@ -44,20 +44,25 @@ namespace {
 
 constexpr int kWarps = 4;                // of a block on the line, and of the join
 constexpr int kThreads = kWarps * 32;
-constexpr int kStripWarps = 8;           // of a strip's block
+constexpr int kStripWarps = 8;           // of a strip's block where there are few strips
 constexpr float kGrow = 4.0f;  // how far (log2) a score may pass the running maximum
 constexpr int kGrowV = 3;      // the same for V's powers of two
 
-// Tables of up to so many pages take a block a strip: 1 sequence of 512 tokens STRIP1 us against 8.4 with
+// Tables of up to so many pages take a block a strip: 1 sequence of 512 tokens 7.2 us against 8.4 with
 // the line, whose scan and join cost about 4 us.
 constexpr int kStripPages = 64;
 
+// How the blocks share the work: a run of the line each, or a strip each with kWarps or kStripWarps warps.
+enum Mode { kLine, kStrip, kWideStrip };
+
 // Warps of a block, pages of a warp's ring, and blocks a multiprocessor (registers and rings together).
-template <bool E4M3, int NT, bool LINE>
+template <bool E4M3, int NT, Mode MODE>
 struct Shape {
-    static constexpr int kWarps = LINE ? q3::kWarps : kStripWarps;
-    static constexpr int kStages = E4M3 && !LINE ? 3 : 2;
-    static constexpr int kBlocks = LINE ? (NT == 1 ? (E4M3 ? 5 : 3) : (E4M3 ? 4 : 3)) : (E4M3 ? (NT == 1 ? 2 : 1) : 1);
+    static constexpr int kWarps = MODE == kWideStrip ? kStripWarps : q3::kWarps;
+    static constexpr int kStages = 2;
+    static constexpr int kBlocks = MODE == kLine    ? (NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2))
+                                   : MODE == kStrip ? (NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2))
+                                                    : (NT == 1 && E4M3 ? 2 : 1);
 };
 
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from) {
@@ -241,30 +246,33 @@ __device__ __forceinline__ long long seq_units(const PagedArgs& a, const SeqShap
     return static_cast<long long>(a.n_kv) * row_groups<NT>(s, a.group) * strip_units(seq_pages(s));
 }
 
-// Units of one block's run.
+// Units of one block's run. (Longer runs for the blocks that come first on their multiprocessor and get
+// ahead, their warps being the oldest, were measured and gained nothing.)
 __device__ __forceinline__ long long run_length(long long total, unsigned blocks) {
     return max(static_cast<long long>(kMinUnits), (total + blocks - 1) / static_cast<long long>(blocks));
 }
 
-template <int D, bool E4M3, int NT, bool LINE>
+template <int D, bool E4M3, int NT, Mode MODE>
 struct OwnSmem {
     static constexpr int kRow = E4M3 ? D : 2 * D;                  // bytes of a pool row
     static constexpr int kPage = 2 * kPageTokens * kRow + (E4M3 ? 2 * kPageTokens : 0);  // K, V, bytes
-    static constexpr int kRing = Shape<E4M3, NT, LINE>::kWarps * Shape<E4M3, NT, LINE>::kStages * kPage;
-    static constexpr int kSums = Shape<E4M3, NT, LINE>::kWarps * 8 * NT * D * 4;          // after a run of pages, in its place
+    static constexpr int kRing = Shape<E4M3, NT, MODE>::kWarps * Shape<E4M3, NT, MODE>::kStages * kPage;
+    static constexpr int kSums = Shape<E4M3, NT, MODE>::kWarps * 8 * NT * D * 4;          // after a run of pages, in its place
     static constexpr int kBytes = kRing > kSums ? kRing : kSums;
 };
 
-// LINE: the block takes its run of the line of units. Else it takes one strip and finishes its rows, the
-// prefix's parts among them.
-template <int D, bool E4M3, int NT, bool LINE>
-__global__ void __launch_bounds__(Shape<E4M3, NT, LINE>::kWarps * 32, Shape<E4M3, NT, LINE>::kBlocks)
+// kLine: the block takes its run of the line of units. Else it takes one strip and finishes its rows,
+// the prefix's parts among them.
+template <int D, bool E4M3, int NT, Mode MODE>
+__global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3, NT, MODE>::kBlocks)
     own_pages_kernel(const PagedArgs a) {
     constexpr int MT = D / 16;                    // m-tiles of O^T, k-steps of S^T
+    constexpr int KW = E4M3 ? D / 16 : D / 8;     // words a lane holds of one K row
     constexpr int VW = E4M3 ? D / 32 : D / 16;    // and of one V row
-    using L = OwnSmem<D, E4M3, NT, LINE>;
-    constexpr int W = Shape<E4M3, NT, LINE>::kWarps;
-    constexpr int ROW = L::kRow, PIECES = ROW / 16, STAGES = Shape<E4M3, NT, LINE>::kStages;
+    using L = OwnSmem<D, E4M3, NT, MODE>;
+    constexpr int W = Shape<E4M3, NT, MODE>::kWarps;
+    constexpr bool LINE = MODE == kLine;
+    constexpr int ROW = L::kRow, PIECES = ROW / 16, STAGES = Shape<E4M3, NT, MODE>::kStages;
     constexpr int ROWS = 8 * NT;
     extern __shared__ __align__(128) uint8_t ring_s[];
     float (*o_s)[ROWS][D] = reinterpret_cast<float (*)[ROWS][D]>(ring_s);
@@ -282,7 +290,7 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, LINE>::kWarps * 32, Shape<E4M3
     int b, h, rg, ids = -1;
     if constexpr (LINE) {
         // This block's run of units.
-        const int per_thread = (a.n_seqs + W * 32 - 1) / W * 32;
+        const int per_thread = (a.n_seqs + W * 32 - 1) / (W * 32);
         const int b0 = min(tid * per_thread, a.n_seqs), b1 = min(b0 + per_thread, a.n_seqs);
         auto units = [&](int i) { return seq_units<NT>(a, seq_shape(a, i)); };
         long long mine = 0, before, total;
@@ -383,6 +391,7 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, LINE>::kWarps * 32, Shape<E4M3
         uint32_t qw[NT][D / 8];
         float c_col[E4M3 ? NT : 1][2];  // score factor of the columns 2t, 2t + 1 (a bf16 pool has one for all)
         c_col[0][0] = scale;
+        int seen[NT][2];  // keys that their rows see, none for a row past the last
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int r = r_base + n * 8 + g;
@@ -428,16 +437,21 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, LINE>::kWarps * 32, Shape<E4M3
 #pragma unroll
                 for (int x = 0; x < 2; ++x) c_col[n][x] = __shfl_sync(0xffffffffu, c, (2 * t + x) * 4);
             }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int rr = n * 8 + 2 * t + x;
+                seen[n][x] = rr < n_rows ? s.len - s.rows + (r_base + rr) / a.group + 1 : 0;
+            }
         }
         const int tail_key = s.len - s.rows + r_base / a.group + 1;  // seen by every row below it
 
-        float m[NT][2], neg[NT][2], l[NT][2], o[NT][MT][4];  // neg = kShift - m
+        float m[NT][2], lim[NT][2], neg[NT][2], l[NT][2], o[NT][MT][4];  // lim = m + kGrow, neg = kShift - m
         int r_v = -1000;  // power of two that o is relative to
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                m[n][x] = -INFINITY;
+                m[n][x] = lim[n][x] = -INFINITY;
                 neg[n][x] = kShift;
                 l[n][x] = 0.0f;
             }
@@ -454,37 +468,33 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, LINE>::kWarps * 32, Shape<E4M3
             if (it + STAGES - 1 < steps) start_page(it + STAGES - 1);
             copy_commit();
             constexpr int SW = PIECES < 8 ? PIECES - 1 : 7;
-            uint32_t ex[2] = {0, 0};
+            // All of K's pieces at once (two at a time cost 10% more: each product then waits for its read).
+            uint32_t kr[2][KW], ex[2] = {0, 0};
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int j = 0; j < PIECES / 4; ++j) {
+                    lds_16(page_s + (g + 8 * x) * ROW + ((k_piece<PIECES>(t, j) ^ (g & SW)) * 16), &kr[x][4 * j]);
+                }
+            }
             if constexpr (E4M3) {
                 ex[0] = lds_u16(page_s + 2 * kPageTokens * ROW + g * 2);
                 ex[1] = lds_u16(page_s + 2 * kPageTokens * ROW + g * 2 + 16);
             }
             float sc[NT][4];
-            constexpr int PER = E4M3 ? 4 : 2;  // k-steps of a 16-byte piece
-            uint32_t kr[2][2][4];              // this piece and the next, of both keys
-            auto read_k = [&](int j) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    lds_16(page_s + (g + 8 * x) * ROW + ((k_piece<PIECES>(t, j) ^ (g & SW)) * 16), kr[j & 1][x]);
-                }
-            };
-            read_k(0);
 #pragma unroll
             for (int k = 0; k < MT; ++k) {
-                const int j = k / PER, w = k % PER;
-                if (w == 0 && j + 1 < PIECES / 4) read_k(j + 1);
-                const uint32_t (&kp)[2][4] = kr[j & 1];
                 uint32_t f[4];
                 if constexpr (E4M3) {
-                    f[0] = e4m3x2_to_f16x2(kp[0][w]);
-                    f[1] = e4m3x2_to_f16x2(kp[1][w]);
-                    f[2] = e4m3x2_hi_to_f16x2(kp[0][w]);
-                    f[3] = e4m3x2_hi_to_f16x2(kp[1][w]);
+                    f[0] = e4m3x2_to_f16x2(kr[0][k]);
+                    f[1] = e4m3x2_to_f16x2(kr[1][k]);
+                    f[2] = e4m3x2_hi_to_f16x2(kr[0][k]);
+                    f[3] = e4m3x2_hi_to_f16x2(kr[1][k]);
                 } else {
-                    f[0] = kp[0][2 * w];
-                    f[1] = kp[1][2 * w];
-                    f[2] = kp[0][2 * w + 1];
-                    f[3] = kp[1][2 * w + 1];
+                    f[0] = kr[0][2 * k];
+                    f[1] = kr[1][2 * k];
+                    f[2] = kr[0][2 * k + 1];
+                    f[3] = kr[1][2 * k + 1];
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -495,22 +505,28 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, LINE>::kWarps * 32, Shape<E4M3
             const bool tail = !there || key0 + kPageTokens > tail_key;
             const int limit = there ? s.len - key0 : 0;  // this page's keys that exist
             float p[NT][4];
-            bool grow = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float x = sc[n][i] * (E4M3 ? c_col[n][i & 1] : c_col[0][0]);
-                    if constexpr (E4M3) x *= __uint_as_float((ex[i >> 1] & 0xffu) << 23);  // 2^(byte - 127)
-                    if (tail) {
-                        // Keys that this column's row sees: none for a row past the last.
-                        const int rr = n * 8 + 2 * t + (i & 1);
-                        const int seen = there && rr < n_rows ? s.len - s.rows + (r_base + rr) / a.group + 1 : 0;
-                        if (key0 + g + 8 * (i >> 1) >= seen) x = -INFINITY;
-                    }
-                    p[n][i] = x;
-                    grow |= x > m[n][i & 1] + kGrow;
+                    p[n][i] = sc[n][i] * (E4M3 ? c_col[n][i & 1] : c_col[0][0]);
+                    if constexpr (E4M3) p[n][i] *= __uint_as_float((ex[i >> 1] & 0xffu) << 23);  // 2^(byte - 127)
                 }
+            }
+            if (tail) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (!there || key0 + g + 8 * (i >> 1) >= seen[n][i & 1]) p[n][i] = -INFINITY;
+                    }
+                }
+            }
+            bool grow = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) grow |= p[n][i] > lim[n][i & 1];
             }
             int v_top = 0;
             if constexpr (E4M3) {
@@ -538,6 +554,7 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, LINE>::kWarps * 32, Shape<E4M3
                         const float m_new = fmaxf(m[n][x], mx);
                         f[x] = m_new == m[n][x] ? 1.0f : ex2(m[n][x] - m_new);
                         m[n][x] = m_new;
+                        lim[n][x] = m_new + kGrow;
                         neg[n][x] = kShift - (m_new == -INFINITY ? 0.0f : m_new);
                         l[n][x] *= f[x];
                         f[x] *= fv;
@@ -818,25 +835,31 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const PagedArgs a, const
         a.f16);
 }
 
+template <int D, bool E4M3, int NT, Mode MODE>
+void launch_strips(const PagedArgs& a, long long strips, cudaStream_t s) {
+    constexpr int bytes = OwnSmem<D, E4M3, NT, MODE>::kBytes;
+    auto kernel = own_pages_kernel<D, E4M3, NT, MODE>;
+    Q3_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    launch_dep(a.prefix_len > 0, kernel, dim3(static_cast<unsigned>(strips)),
+               dim3(Shape<E4M3, NT, MODE>::kWarps * 32), bytes, s, a);
+}
+
 template <int D, bool E4M3, int NT>
 void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
     const long long groups = (static_cast<long long>(a.max_q) * a.group + 8 * NT - 1) / (8 * NT);
     const long long strips = static_cast<long long>(a.n_seqs) * a.n_kv * groups;
     if (a.table_stride <= kStripPages) {
         // Short sequences: a block a strip, no line to find and nothing to join after it.
-        constexpr int bytes = OwnSmem<D, E4M3, NT, false>::kBytes;
-        auto kernel = own_pages_kernel<D, E4M3, NT, false>;
-        Q3_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-        launch_dep(a.prefix_len > 0, kernel, dim3(static_cast<unsigned>(strips)), dim3(kStripWarps * 32), bytes,
-                   s, a);
+        if (strips <= sms) launch_strips<D, E4M3, NT, kWideStrip>(a, strips, s);
+        else launch_strips<D, E4M3, NT, kStrip>(a, strips, s);
         return;
     }
+    constexpr int per_sm = Shape<E4M3, NT, kLine>::kBlocks, bytes = OwnSmem<D, E4M3, NT, kLine>::kBytes;
     // No more blocks than the table's width could fill.
     const long long most = (strips * (a.table_stride + kSetup) + kMinUnits - 1) / kMinUnits;
     const int grid = static_cast<int>(
-        std::min({most, static_cast<long long>(sms) * Shape<E4M3, NT, true>::kBlocks, static_cast<long long>(kMaxBlocks)}));
-    constexpr int bytes = OwnSmem<D, E4M3, NT, true>::kBytes;
-    auto kernel = own_pages_kernel<D, E4M3, NT, true>;
+        std::min({most, static_cast<long long>(sms) * per_sm, static_cast<long long>(kMaxBlocks)}));
+    auto kernel = own_pages_kernel<D, E4M3, NT, kLine>;
     Q3_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     launch_dep(a.prefix_len > 0, kernel, dim3(grid), dim3(kThreads), bytes, s, a);
     const long long rows = static_cast<long long>(a.n_seqs) * a.n_kv * a.max_q * a.group;

@@ -31,7 +31,7 @@ struct PagedArgs {
 };
 
 constexpr float kShift = 8.0f;     // the weights' largest is about 2^8: fp16 then reaches to 2^-32 of it
-constexpr int kMaxBlocks = 760;    // of the line: at least 5 a multiprocessor
+constexpr int kMaxBlocks = 640;    // of the line: at least 4 a multiprocessor
 constexpr int kSetup = 4;          // what a strip costs beside its pages, in pages
 constexpr int kMinUnits = 8;       // a block's smallest share
 
