@@ -32,7 +32,7 @@ struct PagedArgs {
 
 constexpr float kShift = 8.0f;     // the weights' largest is about 2^8: fp16 then reaches to 2^-32 of it
 constexpr int kMaxBlocks = 640;    // of the line: at least 4 a multiprocessor
-constexpr int kSetup = 4;          // what a strip costs beside its pages, in pages
+constexpr int kSetup = 16;         // what a strip costs beside its pages, in pages (4: 64 sequences 60 us, 8: 56, 16: 54, 24: 55)
 constexpr int kMinUnits = 8;       // a block's smallest share
 
 // Rows of sequence b and its own tokens, whatever the arrays hold.
