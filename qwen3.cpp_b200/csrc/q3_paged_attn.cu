@@ -396,8 +396,9 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
         for (int n = 0; n < NT; ++n) {
             const int r = r_base + n * 8 + g;
             const bool live = n * 8 + g < n_rows;
+            const int token = token_of(a, r);
             const uint16_t* qp = static_cast<const uint16_t*>(a.q) +
-                                 (live ? (s.row0 + r / a.group) * a.q_stride + (h * a.group + r % a.group) * D : 0);
+                                 (live ? (s.row0 + token) * a.q_stride + (h * a.group + r - token * a.group) * D : 0);
             constexpr int CH = E4M3 ? 16 : 8;  // values of a 16-byte piece
 #pragma unroll
             for (int j = 0; j < PIECES / 4; ++j) {
@@ -440,10 +441,10 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int rr = n * 8 + 2 * t + x;
-                seen[n][x] = rr < n_rows ? s.len - s.rows + (r_base + rr) / a.group + 1 : 0;
+                seen[n][x] = rr < n_rows ? s.len - s.rows + token_of(a, r_base + rr) + 1 : 0;
             }
         }
-        const int tail_key = s.len - s.rows + r_base / a.group + 1;  // seen by every row below it
+        const int tail_key = s.len - s.rows + token_of(a, r_base) + 1;  // seen by every row below it
 
         float m[NT][2], lim[NT][2], neg[NT][2], l[NT][2], o[NT][MT][4];  // lim = m + kGrow, neg = kShift - m
         int r_v = -1000;  // power of two that o is relative to
@@ -729,8 +730,8 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
                         ml = a.prefix_ml + i * split + row;
                         o = a.prefix_o + (i * split + row) * D;
                     },
-                    static_cast<uint16_t*>(a.out) + (s.row0 + rr / a.group) * a.out_stride +
-                        (h * a.group + rr % a.group) * D,
+                    static_cast<uint16_t*>(a.out) + (s.row0 + token_of(a, rr)) * a.out_stride +
+                        (h * a.group + rr - token_of(a, rr) * a.group) * D,
                     a.f16);
             }
             break;
@@ -756,8 +757,9 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
             if (whole && a.prefix_len == 0) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees nothing is zeros
                 const int rr = r_base + r;
-                uint16_t* out = static_cast<uint16_t*>(a.out) + (s.row0 + rr / a.group) * a.out_stride +
-                                (h * a.group + rr % a.group) * D + d;
+                const int token = token_of(a, rr);
+                uint16_t* out = static_cast<uint16_t*>(a.out) + (s.row0 + token) * a.out_stride +
+                                (h * a.group + rr - token * a.group) * D + d;
                 *reinterpret_cast<uint2*>(out) = make_uint2(pack2_out(y.x * inv, y.y * inv, a.f16),
                                                             pack2_out(y.z * inv, y.w * inv, a.f16));
             } else if (whole) {
@@ -831,7 +833,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const PagedArgs a, const
                 o = a.own_o + at * D;
             }
         },
-        static_cast<uint16_t*>(a.out) + (s.row0 + r / a.group) * a.out_stride + (h * a.group + r % a.group) * D,
+        static_cast<uint16_t*>(a.out) + (s.row0 + token_of(a, r)) * a.out_stride +
+            (h * a.group + r - token_of(a, r) * a.group) * D,
         a.f16);
 }
 
@@ -950,6 +953,7 @@ void paged_attention(void* out, void* workspace, const void* q, int type, int64_
     a.n_pages = static_cast<int>(pool->n_pages);
     a.n_kv = pool->n_kv_heads;
     a.group = n_heads / pool->n_kv_heads;
+    a.group_magic = a.group == 1 ? 0u : static_cast<unsigned>(((1ull << 32) + a.group - 1) / a.group);
     a.n_q = n_q;
     a.n_seqs = n_seqs;
     a.max_q = max_q;

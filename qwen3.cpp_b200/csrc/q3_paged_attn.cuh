@@ -18,6 +18,7 @@ struct PagedArgs {
     const int32_t* prefix_table;
     long long q_stride, out_stride;
     int n_pages, n_kv, group, n_q, n_seqs, max_q, table_stride, prefix_len;
+    unsigned group_magic;  // ceil(2^32 / group), 0 for a group of one: see token_of
     int f16;         // q and out are fp16 (else bf16)
     // Workspace. Partial results are in fp32: o = sum p v and (m, l) = (max of the scores in units of
     // log2, sum p), p = 2^(score - m + kShift).
@@ -33,7 +34,7 @@ struct PagedArgs {
 constexpr float kShift = 8.0f;     // the weights' largest is about 2^8: fp16 then reaches to 2^-32 of it
 constexpr int kMaxBlocks = 640;    // of the line: at least 4 a multiprocessor
 constexpr int kSetup = 16;         // what a strip costs beside its pages, in pages (4: 64 sequences 60 us, 8: 56, 16: 54, 24: 55)
-constexpr int kMinUnits = 8;       // a block's smallest share
+constexpr int kMinUnits = 12;      // a block's smallest share
 
 // Rows of sequence b and its own tokens, whatever the arrays hold.
 struct SeqShape {
@@ -49,7 +50,12 @@ __device__ __forceinline__ SeqShape seq_shape(const PagedArgs& a, int b) {
     return s;
 }
 
-// Row r of (sequence, KV head): query token r / group, query head r % group of the KV head's.
+// The query token of row r of a KV head, r / group (its head of the group is r % group): exact for rows
+// below 2^26, as magic * group is less than 2^32 + 64.
+__device__ __forceinline__ int token_of(const PagedArgs& a, int r) {
+    return a.group_magic ? static_cast<int>(__umulhi(static_cast<unsigned>(r), a.group_magic)) : r;
+}
+
 __device__ __forceinline__ int seq_pages(const SeqShape& s) {
     return static_cast<int>((static_cast<long long>(s.len) + kPageTokens - 1) / kPageTokens);
 }

@@ -300,18 +300,30 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
             commit();
         }
     }
-    // ---------------------------------------------------------------- softmax: this thread's row of Q
+    // ---------------------------------------------------------------- softmax: the rows of Q on their way
+    // Whole rows, Q_LANES lanes each, into their places in the operand (a thread reading its own row from
+    // global memory touches 32 lines an instruction: 2 us for the CTA).
+    constexpr int Q_LANES = D / 8, Q_ROWS = 32 / Q_LANES;
     const int s = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
-    const int row = row_base + (PAIR ? s * kRowTile : 0) + r;
+    const int tile_row = row_base + (PAIR ? s * kRowTile : 0);
+    const int row = tile_row + r;
     const bool live = warp < 8 && row < rows;
-    uint4 q[D / 8];
+    uint8_t* q_tile = sm + L::kQ + (PAIR ? s * L::kTile : 0);
     if (warp < 8) {
-        const uint16_t* p = static_cast<const uint16_t*>(a.q) +
-                            (live ? row / a.group * a.q_stride + (h * a.group + row % a.group) * D : 0);
+        const int piece = lane % Q_LANES;
+        // SOLO: the two streams' warps bring half of the one tile's rows each.
+        const int first = (warp & 3) * 32 + (PAIR ? 0 : s * 16), n_rows = PAIR ? 32 : 16;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-            q[i] = live ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < n_rows; i += Q_ROWS) {
+            const int qr = first + i + lane / Q_LANES, token = token_of(a, tile_row + qr);
+            const bool in = tile_row + qr < rows;
+            const uint16_t* from = static_cast<const uint16_t*>(a.q) + piece * 8 +
+                                   (in ? token * a.q_stride + (h * a.group + tile_row + qr - token * a.group) * D : 0);
+            uint8_t* to = q_tile + qr * 128 + (piece >> 3) * kPanel + (((piece & 7) ^ (qr & 7)) * 16);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(in ? 16 : 0)
+                         : "memory");
         }
+        commit();
     }
 
     // The CTA's pages and the largest bytes of their keys: a thread a page, the first of its pages looked
@@ -540,10 +552,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
         // ---------------------------------------------------------------- softmax
         more_registers<kManyRegs>();
         float c = 1.4426950408889634f / sqrtf(static_cast<float>(D));
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        softmax_sync();
         if constexpr (E4M3) {
-            // The row scaled by a power of two for fp16.
-            uint32_t* w = reinterpret_cast<uint32_t*>(q);
+            // This thread's row, scaled by a power of two for fp16.
+            uint8_t* line = q_tile + r * 128;
+            alignas(16) uint32_t w[D / 2];
             float big = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                *reinterpret_cast<uint4*>(w + 4 * i) =
+                    *reinterpret_cast<const uint4*>(line + (i >> 3) * kPanel + (((i & 7) ^ (r & 7)) * 16));
+            }
 #pragma unroll
             for (int i = 0; i < D / 2; ++i) {
                 big = max3(big, fabsf(a.f16 ? f16_lo(w[i]) : bf16_lo(w[i])),
@@ -553,21 +573,24 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
             if (big > 0.0f && big < INFINITY) {
                 e = min(13 + 127 - static_cast<int>(__float_as_uint(big) >> 23), 126);
             }
-            const float f = pow2(e);
-#pragma unroll
-            for (int i = 0; i < D / 2; ++i) {
-                w[i] = pack2_out((a.f16 ? f16_lo(w[i]) : bf16_lo(w[i])) * f,
-                                 (a.f16 ? f16_hi(w[i]) : bf16_hi(w[i])) * f, 1);
-            }
             // Kept a normal number: a masked score is -infinity times it.
             c = fminf(fmaxf(c * pow2(-e) * exp_of_byte(static_cast<uint32_t>(top_k)), 1e-37f), 1e37f);
+            if constexpr (!PAIR) softmax_sync();  // both streams have read the row
+            if (PAIR || s == 0) {
+                const float f = pow2(e);
+#pragma unroll
+                for (int i = 0; i < D / 2; ++i) {
+                    w[i] = pack2_out((a.f16 ? f16_lo(w[i]) : bf16_lo(w[i])) * f,
+                                     (a.f16 ? f16_hi(w[i]) : bf16_hi(w[i])) * f, 1);
+                }
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    *reinterpret_cast<uint4*>(line + (i >> 3) * kPanel + (((i & 7) ^ (r & 7)) * 16)) =
+                        *reinterpret_cast<const uint4*>(w + 4 * i);
+                }
+            }
         }
         if (PAIR || s == 0) {
-            uint8_t* to = sm + L::kQ + (PAIR ? s * L::kTile : 0) + r * 128;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                *reinterpret_cast<uint4*>(to + (i >> 3) * kPanel + (((i & 7) ^ (r & 7)) * 16)) = q[i];
-            }
             fence_smem_to_mma();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
