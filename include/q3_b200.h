@@ -427,7 +427,7 @@ q3_status q3_paged_attn(void* out, void* workspace, const void* q, int type, int
 /* q3_paged_attn where the prefix_len tokens of prefix_table's pages come before every sequence's own
  * tokens and are seen by every row: their keys are read once for the rows of all sequences, as
  * tensor-core contractions (tcgen05), and joined with each sequence's own part by the softmax
- * statistics. prefix_len may be any number (the last page need not be full); kv_len counts a
+ * statistics. prefix_len may be any number up to 2^28 (the last page need not be full); kv_len counts a
  * sequence's own tokens alone and may be 0. The workspace is sized with this prefix_len. A
  * tensor-core pipeline wait that gives up (it is bounded) leaves NaN in the rows of its part. */
 q3_status q3_prefix_attn(void* out, void* workspace, const void* q, int type, int64_t q_stride,

@@ -878,12 +878,12 @@ void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
 
 // ------------------------------------------------------------------ host
 
-constexpr int kMaxGroup = 64, kMaxRows = 128, kMaxBatchRows = 1 << 23;
+constexpr int kMaxGroup = 64, kMaxRows = 128, kMaxBatchRows = 1 << 23, kMaxPrefix = 1 << 28;
 
 bool sizes_ok(const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs, int max_q, int prefix_len) {
     return n_heads > 0 && n_heads % pool->n_kv_heads == 0 && n_heads / pool->n_kv_heads <= kMaxGroup &&
            n_q >= 0 && n_seqs >= 0 && max_q > 0 &&
-           static_cast<long long>(max_q) * (n_heads / pool->n_kv_heads) <= kMaxRows && prefix_len >= 0 &&
+           static_cast<long long>(max_q) * (n_heads / pool->n_kv_heads) <= kMaxRows && prefix_len >= 0 && prefix_len <= kMaxPrefix &&
            static_cast<long long>(n_q) * (n_heads / pool->n_kv_heads) <= kMaxBatchRows &&
            static_cast<long long>(n_seqs) * max_q * n_heads <= INT_MAX;
 }

@@ -300,7 +300,7 @@ extern "C" q3_status q3_verify_drafts(int32_t* tokens, int32_t* n_accepted, cons
                                       const float* u_sample, int n_seqs, int max_drafts, int vocab,
                                       void* stream) {
     return q3::guard([&] {
-        if (n_seqs < 0 || max_drafts < 0 || max_drafts > 1024 || vocab <= 0) {
+        if (n_seqs < 0 || max_drafts < 0 || max_drafts > 1024 || vocab <= 0 || vocab > (1 << 30)) {
             throw std::invalid_argument("draft verification: size out of range");
         }
         if (n_seqs == 0) return;

@@ -411,6 +411,95 @@ def test_offsets_past_32_bits(T, q3lib, kind, typ):
     small.check()
 
 
+@pytest.mark.parametrize("kind,typ", KINDS)
+@pytest.mark.parametrize("prefix", [0, 150])
+@pytest.mark.parametrize("width", [None, 0, 70])
+def test_rows_between_sequences_and_odd_tables(T, q3lib, kind, typ, prefix, width):
+    """q_start begins past 0 and leaves rows out; tables without a page, and wider than any sequence."""
+    lens = [0, 0, 0] if width == 0 else [20, 33, 7]
+    b = Batch(T, q3lib, kind, typ, 2, 3, 128, lens, [2, 1, 2], prefix=prefix, seed=17, spare_rows=6)
+    # Rows 1, 2 | 4 | 6 of the buffer; the third sequence ends where it would run past the last row.
+    b.q_start.copy_(T.tensor([1, 3, 4, 6], dtype=T.int32))
+    if width == 0:
+        b.width = 0
+    elif width:
+        wide = T.full((3, width), -9, dtype=T.int32, device="cuda")
+        wide[:, :b.width] = b.table
+        b.table, b.width = wide, width
+    b.starts = [1, 3, 4, 6]
+    b.call()
+    T.cuda.synchronize()
+    val, err = b.want()
+    got = b.out_buf.double()[:, :6 * 128].view(-1, 6, 128)
+    assert bool((got[1:6] - val[1:6]).abs().le(err[1:6] + 2.0 ** -24 * T.finfo(b.dt).tiny).all())
+    assert bool((b.out_buf[0] == 9).all()) and bool((b.out_buf[6:] == 9).all())
+    # A gap: the second sequence has no row, row 3 belongs to nothing.
+    b.out_buf.fill_(9)
+    b.q_start.copy_(T.tensor([1, 3, 3, 5], dtype=T.int32))
+    b.counts, b.starts = [2, 0, 2], [1, 3, 3, 5]
+    b.call()
+    T.cuda.synchronize()
+    val, err = b.want()
+    got = b.out_buf.double()[:, :6 * 128].view(-1, 6, 128)
+    assert bool((got[1:5] - val[1:5]).abs().le(err[1:5] + 2.0 ** -24 * T.finfo(b.dt).tiny).all())
+    assert bool((b.out_buf[0] == 9).all()) and bool((b.out_buf[5:] == 9).all())
+
+
+@pytest.mark.parametrize("kind,typ", KINDS)
+def test_no_prefix_is_the_plain_call(T, q3lib, kind, typ):
+    b = Batch(T, q3lib, kind, typ, 2, 2, 128, [900, 1300, 2], [3, 1, 2], seed=18)
+    b.call()
+    b.check()
+    out = T.full_like(b.out_buf, 9)
+    q3lib.prefix_attn(out.data_ptr(), b.ws.data_ptr(), b.q_buf.data_ptr(), b.code, b.stride, b.stride,
+                      b.pool.handle, 4, b.n_q, 3, b.max_q, b.q_start.data_ptr(), b.kv_len.data_ptr(),
+                      b.table.data_ptr(), b.width, None, 0)
+    T.cuda.synchronize()
+    assert T.equal(out, b.out_buf)
+
+
+@pytest.mark.parametrize("kind,typ", KINDS)
+@pytest.mark.parametrize("h,group,d,counts", [(4, 2, 128, [1, 1, 1]), (2, 5, 64, [2, 3, 1]), (1, 8, 128, [8, 1, 16])])
+def test_long_tables_with_a_prefix(T, q3lib, kind, typ, h, group, d, counts):
+    """Sequences long enough to be cut among blocks, behind a prefix."""
+    b = Batch(T, q3lib, kind, typ, h, group, d, [2300, 9, 1100], counts, prefix=700, seed=19)
+    b.call()
+    b.check()
+
+
+def test_rows_of_nan_and_infinity_stay_their_own(T, q3lib):
+    """A query row that holds NaN or infinity gives NaN in its own rows and leaves the others alone."""
+    for prefix in (0, 300):
+        b = Batch(T, q3lib, "e4m3", "bf16", 2, 2, 128, [40, 40, 40], [1, 1, 1], prefix=prefix, seed=20)
+        val, err = b.want()
+        b.q_buf[0, 5] = math.nan
+        b.q_buf[0, 300] = math.nan
+        b.q_buf[1, ::128] = math.inf
+        b.call()
+        T.cuda.synchronize()
+        got = b.out_buf.double()[:, :512].view(-1, 4, 128)
+        assert bool(got[0, 0].isnan().all()) and bool(got[0, 2].isnan().all()) and bool(got[1].isnan().all())
+        assert bool((got[0, 1::2] - val[0, 1::2]).abs().le(err[0, 1::2]).all())
+        assert bool((got[2] - val[2]).abs().le(err[2]).all())
+
+
+def test_a_nan_key_reaches_the_rows_that_see_it(T, q3lib):
+    for kind in ("e4m3", "bf16"):
+        b = Batch(T, q3lib, kind, "bf16", 2, 2, 128, [40, 40], [1, 1], prefix=300, seed=22)
+        slot = b.prefix_slots[130]
+        page, off = slot // PAGE, slot % PAGE
+        if kind == "e4m3":
+            b.pool.k[page, 1, off, 9] = 0x7F
+        else:
+            b.pool.k[page, 1, off, 9] = math.nan
+        val, err = b.want()
+        b.call()
+        T.cuda.synchronize()
+        got = b.out_buf.double()[:2, :512].view(2, 4, 128)
+        assert bool(got[:, 2:].isnan().all())
+        assert bool((got[:, :2] - val[:2, :2]).abs().le(err[:2, :2]).all())
+
+
 # ------------------------------------------------------------------ streams, graphs, workspaces
 
 @pytest.mark.parametrize("prefix", [0, 500])

@@ -78,7 +78,8 @@ def test_bad_attention_is_refused(q3lib, over):
 
 
 def test_bad_prefix_is_refused(q3lib):
-    for over in (dict(prefix_len=-1), dict(prefix_table=None), dict(prefix_table=P + 2)):
+    for over in (dict(prefix_len=-1), dict(prefix_len=(1 << 28) + 1), dict(prefix_table=None),
+                 dict(prefix_table=P + 2)):
         with pytest.raises(q3lib.InvalidArgument, match="paged attention"):
             _attn(q3lib, _pool(q3lib), True, **over)
 
@@ -107,7 +108,7 @@ VERIFY = dict(tokens=P, n_accepted=P, target=P, t_seq=300, t_row=100, draft=P, d
 
 
 @pytest.mark.parametrize("over", [
-    dict(n_seqs=-1), dict(max_drafts=-1), dict(max_drafts=1025), dict(vocab=0), dict(tokens=None),
+    dict(n_seqs=-1), dict(max_drafts=-1), dict(max_drafts=1025), dict(vocab=0), dict(vocab=(1 << 30) + 1), dict(tokens=None),
     dict(n_accepted=None), dict(target=None), dict(draft_tokens=None), dict(u_accept=None),
     dict(u_sample=None), dict(t_row=99), dict(d_row=99), dict(t_seq=-1), dict(d_seq=-1),
     dict(target=P + 2), dict(tokens=P + 1)], ids=str)
