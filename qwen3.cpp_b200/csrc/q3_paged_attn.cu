@@ -52,6 +52,12 @@ constexpr int kGrowV = 3;      // the same for V's powers of two
 // the line, whose scan and join cost about 4 us.
 constexpr int kStripPages = 64;
 
+// A prefix this short (pages, the sequence's own among them) for this little work (strips x prefix pages)
+// is read by each strip in front of its own pages, from L2 after the first: one launch instead of two.
+// (30 sequences of 2 rows, 4 KV heads, 300 shared tokens: 7.8 us against 15.1; 100 of 1 row, 8 heads, 160
+// tokens: 16.9 against 22.1; 1000 tokens, past the limit: 40 against 24.)
+constexpr int kInlinePages = 96, kInlineWork = 16384;
+
 // How the blocks share the work: a run of the line each, or a strip each with kWarps or kStripWarps warps.
 enum Mode { kLine, kStrip, kWideStrip };
 
@@ -319,13 +325,15 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
         h = static_cast<int>(blockIdx.x / most % a.n_kv);
         b = static_cast<int>(blockIdx.x / most / a.n_kv);
         // The first pages' numbers are on their way with the lengths.
-        const int p = warp + lane * W;
-        if (p < a.table_stride) ids = a.table[static_cast<size_t>(b) * a.table_stride + p];
+        const int p = warp + lane * W - a.inline_pages;
+        if (p < 0) ids = a.prefix_table[p + a.inline_pages];
+        else if (p < a.table_stride) ids = a.table[static_cast<size_t>(b) * a.table_stride + p];
     }
     while (pos < end) {
         const SeqShape s = seq_shape(a, b);
         const int pages = seq_pages(s), groups = row_groups<NT>(s, a.group);
         int p0 = 0, p1 = pages;
+        const int before = LINE ? 0 : a.inline_pages;  // of the prefix, in front of the strip's own
         if constexpr (LINE) {
             const int each = strip_units(pages);
             const long long all = static_cast<long long>(a.n_kv) * groups * each;
@@ -347,6 +355,7 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
         } else {
             pos = end;
             if (rg >= groups) break;
+            p1 += before;
         }
         const int r_base = rg * ROWS;
         const int n_rows = min(ROWS, s.rows * a.group - r_base);
@@ -359,7 +368,7 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
         auto start_page = [&](int it) {  // in order: 0, 1, 2, ...
             if ((it & 31) == 0 && (LINE || it > 0)) {
                 const int p = p0 + warp + (it + lane) * W;
-                ids = p < p1 ? table[p] : -1;
+                ids = p >= p1 ? -1 : p < before ? a.prefix_table[p] : table[p - before];
             }
             const int page = __shfl_sync(0xffffffffu, ids, it & 31);
             const bool in = page >= 0 && page < a.n_pages;
@@ -461,7 +470,9 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
         }
 
         for (int it = 0; it < steps; ++it) {
-            const int key0 = (p0 + warp + it * W) * kPageTokens;
+            const int p_here = p0 + warp + it * W;
+            const bool shared = !LINE && p_here < before;  // a page of the prefix: all rows see all its keys
+            const int key0 = (shared ? p_here : p_here - before) * kPageTokens;
             copy_wait<STAGES - 2>();
             __syncwarp();  // every lane's copies of this page are in, and its reads of the one before done
             // `good` grows a bit a page looked up: this page's is (pages looked up since) from its end.
@@ -503,8 +514,8 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
                     else mma16816<E4M3>(sc[n], f[0], f[1], f[2], f[3], qw[n][2 * k], qw[n][2 * k + 1]);
                 }
             }
-            const bool tail = !there || key0 + kPageTokens > tail_key;
-            const int limit = there ? s.len - key0 : 0;  // this page's keys that exist
+            const bool tail = !there || key0 + kPageTokens > (shared ? a.prefix_len : tail_key);
+            const int limit = there ? (shared ? a.prefix_len : s.len) - key0 : 0;  // this page's keys that exist
             float p[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -519,7 +530,8 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        if (!there || key0 + g + 8 * (i >> 1) >= seen[n][i & 1]) p[n][i] = -INFINITY;
+                        const int k = g + 8 * (i >> 1);
+                        if (k >= limit || (!shared && key0 + k >= seen[n][i & 1])) p[n][i] = -INFINITY;
                     }
                 }
             }
@@ -630,7 +642,7 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
                     // that the token does not see as zeros.
                     const int first = r_base / a.group, last = (r_base + n_rows - 1) / a.group;
                     for (int tok = first; tok <= last; ++tok) {
-                        const int lim = there ? s.len - s.rows + tok + 1 - key0 : 0;
+                        const int lim = shared ? limit : there ? s.len - s.rows + tok + 1 - key0 : 0;
                         uint32_t vm[4][VP];
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
@@ -843,7 +855,7 @@ void launch_strips(const PagedArgs& a, long long strips, cudaStream_t s) {
     constexpr int bytes = OwnSmem<D, E4M3, NT, MODE>::kBytes;
     auto kernel = own_pages_kernel<D, E4M3, NT, MODE>;
     Q3_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    launch_dep(a.prefix_len > 0, kernel, dim3(static_cast<unsigned>(strips)),
+    launch_dep(a.prefix_splits > 0, kernel, dim3(static_cast<unsigned>(strips)),
                dim3(Shape<E4M3, NT, MODE>::kWarps * 32), bytes, s, a);
 }
 
@@ -851,7 +863,7 @@ template <int D, bool E4M3, int NT>
 void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
     const long long groups = (static_cast<long long>(a.max_q) * a.group + 8 * NT - 1) / (8 * NT);
     const long long strips = static_cast<long long>(a.n_seqs) * a.n_kv * groups;
-    if (a.table_stride <= kStripPages) {
+    if (a.inline_pages > 0 || a.table_stride <= kStripPages) {
         // Short sequences: a block a strip, no line to find and nothing to join after it.
         if (strips <= sms) launch_strips<D, E4M3, NT, kWideStrip>(a, strips, s);
         else launch_strips<D, E4M3, NT, kStrip>(a, strips, s);
@@ -963,7 +975,15 @@ void paged_attention(void* out, void* workspace, const void* q, int type, int64_
     lay_out(a, static_cast<uint8_t*>(workspace), pool->head_dim);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool e4m3 = pool->type == Q3_TYPE_E4M3;
-    if (prefix_len > 0) launch_prefix_attention(a, pool->head_dim, e4m3, s);
+    const int strip_rows = max_q * a.group <= 8 ? 8 : 16;
+    const long long strips = static_cast<long long>(n_seqs) * a.n_kv * ((max_q * a.group + strip_rows - 1) / strip_rows);
+    const long long pages = (prefix_len + kPageTokens - 1LL) / kPageTokens;
+    if (pages + table_stride <= kInlinePages && strips * pages <= kInlineWork) {
+        a.inline_pages = static_cast<int>(pages);
+        a.prefix_splits = 0;
+    } else if (prefix_len > 0) {
+        launch_prefix_attention(a, pool->head_dim, e4m3, s);
+    }
     if (pool->head_dim == 64) {
         e4m3 ? launch_own<64, true>(a, on.sm_count(), s) : launch_own<64, false>(a, on.sm_count(), s);
     } else {

@@ -29,6 +29,7 @@ struct PagedArgs {
     float* prefix_o;        // [splits][n_kv][prefix_rows][head_dim]
     float2* prefix_ml;      // [splits][n_kv][prefix_rows]
     int prefix_splits, prefix_rows;
+    int inline_pages;       // of the prefix, where the strips read them themselves (prefix_splits is 0 then)
 };
 
 constexpr float kShift = 8.0f;     // the weights' largest is about 2^8: fp16 then reaches to 2^-32 of it
