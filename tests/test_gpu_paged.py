@@ -201,6 +201,14 @@ class Batch:
         # Garbage in the workspace, and a guard behind it.
         self.ws = T.full((size + 256,), 0xFF, dtype=T.uint8, device="cuda")
 
+    def widen(self, width):
+        """The same sequences in a wider table, as one sized for longer ones."""
+        T = self.T
+        wide = T.full((len(self.lens), width), -9, dtype=T.int32, device="cuda")
+        wide[:, :self.width] = self.table
+        self.table, self.width = wide, width
+        return self
+
     def call(self, stream=None, ws=None, out=None):
         args = [(self.out_buf if out is None else out).data_ptr(),
                 (self.ws if ws is None else ws).data_ptr(), self.q_buf.data_ptr(), self.code,
@@ -305,6 +313,57 @@ def test_prefix_attention_row_tiles(T, q3lib, kind, typ, seqs, rows, h, group, p
               prefix=prefix, seed=seqs)
     b.call()
     b.check()
+
+
+@pytest.mark.parametrize("kind,typ", KINDS)
+@pytest.mark.parametrize("prefix", [1, 15, 16, 17, 127, 128, 129, 257, 1003])
+@pytest.mark.parametrize("h,group,d", [(2, 2, 128), (3, 5, 64)])
+def test_prefix_attention_behind_wide_tables(T, q3lib, kind, typ, prefix, h, group, d):
+    """Tables wide enough that a short prefix too goes to the tensor cores."""
+    b = Batch(T, q3lib, kind, typ, h, group, d, [0, 1, 40, 7, 130], [1, 1, 3, 0, 2], prefix=prefix,
+              seed=prefix + d).widen(100)
+    b.call()
+    b.check()
+
+
+@pytest.mark.parametrize("kind,typ", KINDS)
+@pytest.mark.parametrize("seqs,rows,h,group,prefix", [(1, 1, 8, 2, 300), (129, 2, 1, 1, 260), (3, 2, 1, 64, 200),
+                                                      (64, 1, 2, 2, 4099)])
+def test_prefix_row_tiles_behind_wide_tables(T, q3lib, kind, typ, seqs, rows, h, group, prefix):
+    lens = [(7 * i) % 90 for i in range(seqs)]
+    b = Batch(T, q3lib, kind, typ, h, group, 128, lens, [rows - (i % 4 == 3) for i in range(seqs)],
+              prefix=prefix, seed=seqs).widen(101)
+    b.call()
+    b.check()
+
+
+@pytest.mark.parametrize("kind,typ", KINDS)
+@pytest.mark.parametrize("wide", [False, True])
+def test_prefix_of_bad_pages_alone(T, q3lib, kind, typ, wide):
+    """A prefix none of whose pages is in the pool is no prefix."""
+    b = Batch(T, q3lib, kind, typ, 2, 2, 128, [100, 0, 3], [2, 1, 1], prefix=200, seed=24)
+    if wide:
+        b.widen(99)
+    b.prefix_table.fill_(b.pool.n_pages)
+    b.call()
+    b.check(gone=b.prefix_slots.tolist())
+
+
+@pytest.mark.parametrize("kind,typ", KINDS)
+def test_extremes_behind_wide_tables(T, q3lib, kind, typ):
+    """Shared rows of zeros, of 2^-30 and of 2^24 beside ordinary ones, and bad pages among them."""
+    b = Batch(T, q3lib, kind, typ, 2, 2, 128, [60, 200], [2, 3], prefix=300, seed=25, q_scale=1.0).widen(98)
+    k, v = b.pool.get("k", b.prefix_slots), b.pool.get("v", b.prefix_slots)
+    v[0] *= 2.0 ** -30
+    v[1] = 0
+    v[3] *= 2.0 ** (6 if typ == "f16" else 24)
+    v[140] *= 2.0 ** -18
+    k[5], k[6] = 0, k[6] * 2.0 ** -20
+    k[0] = 4 * b.q_buf[3].double().view(2, 2, 128).mean(1)
+    b.pool.put(b.prefix_slots, k, v)
+    b.prefix_table[4] = -1
+    b.call()
+    b.check(gone=b.prefix_slots[64:80].tolist())
 
 
 @pytest.mark.parametrize("kind,typ", KINDS)
@@ -423,9 +482,7 @@ def test_rows_between_sequences_and_odd_tables(T, q3lib, kind, typ, prefix, widt
     if width == 0:
         b.width = 0
     elif width:
-        wide = T.full((3, width), -9, dtype=T.int32, device="cuda")
-        wide[:, :b.width] = b.table
-        b.table, b.width = wide, width
+        b.widen(width)
     b.starts = [1, 3, 4, 6]
     b.call()
     T.cuda.synchronize()
@@ -502,9 +559,9 @@ def test_a_nan_key_reaches_the_rows_that_see_it(T, q3lib):
 
 # ------------------------------------------------------------------ streams, graphs, workspaces
 
-@pytest.mark.parametrize("prefix", [0, 500])
-def test_same_bits_on_any_stream_and_again(T, q3lib, prefix):
-    b = Batch(T, q3lib, "e4m3", "bf16", 4, 2, 128, [900, 40, 333], [2, 1, 3], prefix=prefix, seed=12)
+@pytest.mark.parametrize("prefix,width", [(0, 60), (0, 90), (500, 60), (500, 90)])
+def test_same_bits_on_any_stream_and_again(T, q3lib, prefix, width):
+    b = Batch(T, q3lib, "e4m3", "bf16", 4, 2, 128, [900, 40, 333], [2, 1, 3], prefix=prefix, seed=12).widen(width)
     b.call()
     b.check()
     first = b.out_buf.clone()
@@ -519,10 +576,10 @@ def test_same_bits_on_any_stream_and_again(T, q3lib, prefix):
     assert all(T.equal(first, out) for out in outs)
 
 
-@pytest.mark.parametrize("prefix", [0, 300])
-def test_captured_step_follows_its_lengths(T, q3lib, prefix):
+@pytest.mark.parametrize("prefix,width", [(0, 30), (0, 90), (300, 30), (300, 90)])
+def test_captured_step_follows_its_lengths(T, q3lib, prefix, width):
     """Two graphs over one workspace, replayed in turn, each with lengths and rows set afterwards."""
-    b = Batch(T, q3lib, "e4m3", "f16", 2, 2, 128, [400, 90], [2, 2], prefix=prefix, seed=13)
+    b = Batch(T, q3lib, "e4m3", "f16", 2, 2, 128, [400, 90], [2, 2], prefix=prefix, seed=13).widen(width)
     b.call()  # as a program's eager warm-up
     T.cuda.synchronize()
     stream = T.cuda.Stream()
