@@ -167,6 +167,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     __shared__ int accepted_s;
     const int b = blockIdx.x / a.ctas, rank = blockIdx.x % a.ctas;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n_warps = blockDim.x >> 5;
+    // Another CTA's shared memory may be written once that CTA has started: waited for in front of the writes.
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const int32_t* tok = a.draft_tokens + static_cast<size_t>(b) * a.max_drafts;
     int count = a.max_drafts;
     if (a.max_drafts && a.n_drafts) count = a.n_drafts[b];
@@ -211,6 +213,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     for (int attempt = 0; attempt < 2; ++attempt) {
         const Piece mine = vec ? sum_piece<4, kUnroll>(row, i0, i1) : sum_piece<1, kUnroll>(row, i0, i1);
         if (lane == 0) warps_s[warp] = mine;
+        if (attempt == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         __syncthreads();
         if (warp == 0) {
             Piece all{0.0, -1};
