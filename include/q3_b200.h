@@ -409,9 +409,9 @@ q3_status q3_kv_read(const q3_kv_pool* pool, void* k, void* v, int type, int64_t
  * b has query rows q_start[b] .. q_start[b+1]-1 (at most max_q; q_start[0] >= 0, ascending, at most
  * n_q) and kv_len[b] cached tokens, its rows being the last of them: row i of its n_b sees tokens
  * 0 .. kv_len[b] - n_b + i. One row a sequence is a decode step, more are drafted tokens. Token t of
- * sequence b lies in page table[b * table_stride + t / 16]; kv_len[b] is at most 16 * table_stride. A
- * table entry outside the pool takes its 16 tokens out of the attention. A row that sees nothing is
- * zeros. Rows that belong to no sequence are left as they were.
+ * sequence b lies in page table[b * table_stride + t / 16]; kv_len[b] is at most 16 * table_stride, and
+ * table_stride at most 2^26. A table entry outside the pool takes its 16 tokens out of the attention.
+ * A row that sees nothing is zeros. Rows that belong to no sequence are left as they were.
  * q and out: rows of n_heads heads of head_dim values, q_stride / out_stride elements apart, type BF16
  * (either pool) or F16 (an e4m3 pool), 16-byte aligned; n_heads a multiple of pool->n_kv_heads, at
  * most 64 query heads per KV head; scores are divided by sqrt(head_dim). max_q * n_heads /
@@ -427,9 +427,11 @@ q3_status q3_paged_attn(void* out, void* workspace, const void* q, int type, int
 /* q3_paged_attn where the prefix_len tokens of prefix_table's pages come before every sequence's own
  * tokens and are seen by every row: their keys are read once for the rows of all sequences, as
  * tensor-core contractions (tcgen05), and joined with each sequence's own part by the softmax
- * statistics. prefix_len may be any number up to 2^28 (the last page need not be full); kv_len counts a
- * sequence's own tokens alone and may be 0. The workspace is sized with this prefix_len. A
- * tensor-core pipeline wait that gives up (it is bounded) leaves NaN in the rows of its part. */
+ * statistics. (A prefix of up to 96 pages, table_stride among them, is read by each sequence in front
+ * of its own tokens where the batch is small: one launch instead of two.) prefix_len may be any number
+ * up to 2^28 (the last page need not be full); kv_len counts a sequence's own tokens alone and may be 0.
+ * The workspace is sized with this prefix_len. A tensor-core pipeline wait that gives up (it is bounded)
+ * leaves NaN in the rows of its part. */
 q3_status q3_prefix_attn(void* out, void* workspace, const void* q, int type, int64_t q_stride,
                          int64_t out_stride, const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs,
                          int max_q, const int32_t* q_start, const int32_t* kv_len,

@@ -1,17 +1,18 @@
 // q3_paged_attn / q3_prefix_attn: attention of a ragged batch's newest rows over a paged KV pool,
 // with or without a prefix that every sequence shares.
 //
-// own_pages_kernel computes the part over each sequence's own pages, join_kernel joins the parts.
+// own_pages_kernel computes the part over each sequence's own pages (and over a short prefix, whose pages
+// then stand in front of them), join_kernel joins parts.
 //
-// Work: a strip is the pages of one (sequence, KV head, group of 8 * NT rows); its units are its pages
-// and kSetup more in front, for what a strip costs before and after its pages. The units of all
-// sequences form one line, cut into equal runs, one a block, so a ragged batch loads every block
-// alike and a long sequence spreads over many. Each block finds its run from the lengths on the
-// device (a scan over the sequences), so a captured graph follows them. A strip whose pages lie
-// inside one run is finished there; one that is cut leaves a part per block, at most two a block, and
-// join_kernel adds them by their softmax statistics.
+// Work: a strip is the pages of one (sequence, KV head, group of 8 * NT rows). Where tables are short
+// each strip is one block's, which finishes its rows. Else a strip's units are its pages and kSetup more
+// in front, for what a strip costs before and after its pages. The units of all sequences form one line,
+// cut into equal runs, one a block, so a ragged batch loads every block alike and a long sequence spreads
+// over many. Each block finds its run from the lengths on the device (a scan over the sequences), so a
+// captured graph follows them. A strip whose pages lie inside one run is finished there; one that is cut
+// leaves a part per block, at most two a block, and join_kernel adds them by their softmax statistics.
 //
-// A block's four warps take every fourth page. A page is 16 keys, one m16n8k16 operand tile:
+// A block's warps take a page each in turn. A page is 16 keys, one m16n8k16 operand tile:
 //   S^T[16 keys x 8 rows] = K . Q^T      K's rows are the A operand as they lie in memory
 //   O^T[d x 8 rows]      += V^T . P^T    two keys' V values of one d are a register of A
 // The order of the head's dimensions inside an operand is free as long as both sides agree, so a lane
@@ -19,10 +20,10 @@
 // (e4m3 -> fp16, exact); V pairs need one byte permutation. The scores come out transposed for the
 // second product; movmatrix turns the rounded weights.
 //
-// Each warp has its own ring of kStages pages in shared memory, filled by cp.async a page or two ahead
-// (registers hold one page at most, and the multiprocessor's 16 warps then have too few bytes on the
-// way: 78 us against 67 for 64 sequences of 128 to 4096 tokens). 16-byte piece c of row r lies at
-// piece c ^ (r % 8), which leaves the operand reads without bank conflicts.
+// Each warp has its own ring of two pages in shared memory, filled by cp.async a page ahead (three pages:
+// 64 sequences of 128 to 4096 tokens 56.3 us instead of 53.5, 16 of 5 rows and 100 to 5000 tokens 36.8
+// instead of 37.1). 16-byte piece c of row r lies at piece c ^ (r % 8), which leaves the operand reads
+// without bank conflicts.
 //
 // The running maximum moves only when a score passes it by more than 2^4 (one vote a page instead of
 // two times three shuffles): weights are then at most 2^(kShift + 4), which fp16 holds, as it does 2^3
@@ -32,7 +33,9 @@
 // is in [2^13, 2^14): bf16 and fp16 values are then fp16 values down to 2^-38 of the row's largest.
 // Weights are rounded to fp16 (2^-11), for a bf16 pool to a bf16 pair hi + lo (2^-16). Sums are fp32.
 //
-// Bound by HBM: 2 * (D + 1) bytes a key and KV head (e4m3).
+// Bound by HBM: 2 * (D + 1) bytes a key and KV head (e4m3). 64 sequences of 128 to 4096 tokens, 8 KV heads
+// of 128: 279 MB in 53.5 us, 5.2 TB/s with the start, the last blocks and the join, about 6 TB/s between
+// them; a page costs about 415 warp instructions, which keeps the integer pipe half busy.
 #include <algorithm>
 #include <climits>
 
@@ -55,7 +58,7 @@ constexpr int kStripPages = 64;
 // A prefix this short (pages, the sequence's own among them) for this little work (strips x prefix pages)
 // is read by each strip in front of its own pages, from L2 after the first: one launch instead of two.
 // (30 sequences of 2 rows, 4 KV heads, 300 shared tokens: 7.8 us against 15.1; 100 of 1 row, 8 heads, 160
-// tokens: 16.9 against 22.1; 1000 tokens, past the limit: 40 against 24.)
+// tokens: 16.9 against 22.1; 1000 tokens, past the limit, would take 40 against 24.)
 constexpr int kInlinePages = 96, kInlineWork = 16384;
 
 // How the blocks share the work: a run of the line each, or a strip each with kWarps or kStripWarps warps.
@@ -66,9 +69,8 @@ template <bool E4M3, int NT, Mode MODE>
 struct Shape {
     static constexpr int kWarps = MODE == kWideStrip ? kStripWarps : q3::kWarps;
     static constexpr int kStages = 2;
-    static constexpr int kBlocks = MODE == kLine    ? (NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2))
-                                   : MODE == kStrip ? (NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2))
-                                                    : (NT == 1 && E4M3 ? 2 : 1);
+    static constexpr int kBlocks = MODE == kWideStrip ? (NT == 1 && E4M3 ? 2 : 1)
+                                                      : (NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2));
 };
 
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from) {
@@ -252,8 +254,7 @@ __device__ __forceinline__ long long seq_units(const PagedArgs& a, const SeqShap
     return static_cast<long long>(a.n_kv) * row_groups<NT>(s, a.group) * strip_units(seq_pages(s));
 }
 
-// Units of one block's run. (Longer runs for the blocks that come first on their multiprocessor and get
-// ahead, their warps being the oldest, were measured and gained nothing.)
+// Units of one block's run.
 __device__ __forceinline__ long long run_length(long long total, unsigned blocks) {
     return max(static_cast<long long>(kMinUnits), (total + blocks - 1) / static_cast<long long>(blocks));
 }
@@ -480,7 +481,7 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
             if (it + STAGES - 1 < steps) start_page(it + STAGES - 1);
             copy_commit();
             constexpr int SW = PIECES < 8 ? PIECES - 1 : 7;
-            // All of K's pieces at once (two at a time cost 10% more: each product then waits for its read).
+            // All of K's pieces at once.
             uint32_t kr[2][KW], ex[2] = {0, 0};
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
@@ -787,8 +788,8 @@ __global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3
         }
         __syncthreads();
     }
-    // This grid may have started beside the prefix's, which it does not read; join_kernel waits for this
-    // one alone, so this one ends after that.
+    // On the line this grid may have started beside the prefix's, which it does not read; join_kernel waits
+    // for this one alone, so this one ends after that.
     pdl_wait();
 }
 
@@ -891,6 +892,7 @@ void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
 // ------------------------------------------------------------------ host
 
 constexpr int kMaxGroup = 64, kMaxRows = 128, kMaxBatchRows = 1 << 23, kMaxPrefix = 1 << 28;
+constexpr int kMaxTable = 1 << 26;  // pages: token numbers then stay inside 31 bits
 
 bool sizes_ok(const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs, int max_q, int prefix_len) {
     return n_heads > 0 && n_heads % pool->n_kv_heads == 0 && n_heads / pool->n_kv_heads <= kMaxGroup &&
@@ -931,7 +933,7 @@ void paged_attention(void* out, void* workspace, const void* q, int type, int64_
     if (type != Q3_TYPE_BF16 && !(type == Q3_TYPE_F16 && pool->type == Q3_TYPE_E4M3)) {
         throw std::invalid_argument("paged attention: type must be BF16, or F16 with an e4m3 pool");
     }
-    if (!sizes_ok(pool, n_heads, n_q, n_seqs, max_q, prefix_len) || table_stride < 0) {
+    if (!sizes_ok(pool, n_heads, n_q, n_seqs, max_q, prefix_len) || table_stride < 0 || table_stride > kMaxTable) {
         throw std::invalid_argument("paged attention: size out of range");
     }
     if (n_q == 0 || n_seqs == 0) return;

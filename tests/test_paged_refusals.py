@@ -67,7 +67,7 @@ def _attn(q3, pool, prefix, **over):
 
 @pytest.mark.parametrize("over", [
     dict(type=0), dict(type=3), dict(n_heads=0), dict(n_heads=3), dict(n_heads=130), dict(n_q=-1),
-    dict(n_seqs=-1), dict(max_q=0), dict(max_q=65), dict(table_stride=-1), dict(out=None),
+    dict(n_seqs=-1), dict(max_q=0), dict(max_q=65), dict(table_stride=-1), dict(table_stride=(1 << 26) + 1), dict(out=None),
     dict(ws=None), dict(q=None), dict(q_start=None), dict(kv_len=None), dict(table=None),
     dict(q_stride=511), dict(q_stride=516), dict(out_stride=508), dict(q=P + 8), dict(out=P + 2),
     dict(ws=P + 4), dict(q_start=P + 1), dict(table=P + 2)], ids=str)
