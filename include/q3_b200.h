@@ -381,7 +381,8 @@ q3_status q3_greedy(const float* logits, int n, int32_t* out_index, void* stream
  * for V: the layout of a model's own cache. Slot s is row s % 16 of page s / 16. type Q3_TYPE_BF16:
  * bf16 bits, exps NULL. type Q3_TYPE_E4M3: one byte a value (4 significant bits against bf16's 8,
  * half the bytes), and each row of K and of V has one power of two: exps[page][head][16][2] bytes,
- * K's and V's, and the value is code * 2^(byte - 127). k and v are 16-byte aligned, exps 4-byte. */
+ * K's and V's, at most 254, and the value is code * 2^(byte - 127). k and v are 16-byte aligned, exps
+ * 4-byte. */
 enum { Q3_TYPE_F32 = 0, Q3_TYPE_BF16 = 1, Q3_TYPE_F16 = 2, Q3_TYPE_E4M3 = 3 };
 typedef struct q3_kv_pool {
     void* k;

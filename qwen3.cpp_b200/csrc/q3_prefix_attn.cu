@@ -26,10 +26,10 @@
 // split of the registers), 8-11 loaders, 12 issuer. Every wait is bounded; one that gives up ends the
 // CTA's loops and leaves NaN in its parts.
 //
-// Bound by 4 * D operations a row, head and key for many rows, by HBM for few. 512 rows of 32 heads, 8 KV
-// heads of 128, 32768 keys (e4m3): 0.27 TFLOP in about 250 us, 1.1 PFLOP/s. There a stream's chain (scores,
-// softmax, P into TMEM, product) is longer than the other stream's products, which leaves the tensor pipe
-// 41% busy; the exponentials keep theirs as busy. 8192 keys for 4 rows of each of 16 heads: 15 us.
+// Bound by 4 * D operations a row, head and key for many rows, by latency for few. 427 rows of 32 heads,
+// 8 KV heads of 128, 32768 keys (e4m3): 229 GFLOP in 264 us alone, 0.87 PFLOP/s, the tensor pipe and the
+// exponentials' 41% busy each, shared memory about 68% (scores read 128 bytes a cycle, the loaders write
+// the raw and the converted tiles), the power limit reached. 8192 keys for 64 rows of 16 heads: 18 us.
 #include <algorithm>
 
 #include "q3_paged_attn.cuh"
@@ -780,8 +780,9 @@ void launch(const PagedArgs& a, bool e4m3, cudaStream_t s) {
 
 }  // namespace
 
-// Parts per row. A CTA's time is about (its key tiles + 3), 3 for its start and end; the splits make the
-// sum over the waves of 148 CTAs least.
+// Parts per row. A CTA's time is about (its key tiles + 3), 3 for its start and end (with 5, 8 or 12 the
+// same splits come out at 32768 keys, with 1 others that are 16% slower); the splits make the sum over the
+// waves of 148 CTAs least.
 int prefix_splits(int n_kv, int rows, int prefix_len) {
     if (prefix_len <= 0 || rows <= 0) return 0;
     const bool pair = rows > kRowTile;
