@@ -378,6 +378,15 @@ def test_many_rows_and_many_short_sequences(T, q3lib, kind, typ):
 
 
 @pytest.mark.parametrize("kind,typ", KINDS)
+@pytest.mark.parametrize("prefix,width", [(0, 40), (0, 90), (150, 40), (150, 110)])
+def test_the_largest_group(T, q3lib, kind, typ, prefix, width):
+    """64 query heads to a KV head, two rows a sequence."""
+    b = Batch(T, q3lib, kind, typ, 1, 64, 128, [200, 1, 500], [2, 1, 2], prefix=prefix, seed=17).widen(width)
+    b.call()
+    b.check()
+
+
+@pytest.mark.parametrize("kind,typ", KINDS)
 @pytest.mark.parametrize("prefix", [0, 200])
 def test_bad_pages_leave_the_attention(T, q3lib, kind, typ, prefix):
     b = Batch(T, q3lib, kind, typ, 2, 2, 128, [100, 33, 16], [2, 1, 1], prefix=prefix, seed=8)
@@ -723,6 +732,18 @@ def test_verification_edges(T, q3lib):
     assert got[0][7][0] == 0
 
 
+@pytest.mark.parametrize("b,k,vocab", [(2, 40, 300), (1, 1024, 9), (20, 2, 40000)])
+def test_verification_of_many_drafts(T, q3lib, b, k, vocab):
+    """More drafts than a warp has lanes, all but the last few taken; more blocks than multiprocessors."""
+    target, draft, toks, counts, ua, us = make_verify(T, 77, b, k, vocab)
+    ua[:, :max(1, k - 3)] = 0.0
+    got = run_verify(T, q3lib, target, draft, toks, counts, ua, us, vocab)
+    want = verify_by_hand(target.double().tolist(), draft.double().tolist(), toks.tolist(), counts.tolist(),
+                          ua.double().tolist(), us.double().tolist(), vocab)
+    assert got == (want[0], want[1])
+    assert min(got[1]) >= max(1, k - 3) - 1
+
+
 def test_drawn_tokens_follow_the_target(T, q3lib):
     """Speculative sampling leaves the target's distribution: the first token of 40,000 sequences, each
     cell within 6 standard deviations."""
@@ -775,3 +796,61 @@ def test_a_drafting_step(T, q3lib, prefix):
                               ua.double().tolist(), us.double().tolist(), v)
         assert got == (want[0], want[1])
         lens = [n + 1 + a for n, a in zip(lens, got[1])]
+
+
+def test_all_at_once(T, q3lib):
+    """Every operator on a stream of its own, several rounds on their way together, and once more replayed
+    from one graph that forks to those streams: what each gave alone, to the bit."""
+    own = Batch(T, q3lib, "e4m3", "bf16", 4, 2, 128, [900, 40, 333], [2, 1, 3], seed=41).widen(90)
+    far = Batch(T, q3lib, "bf16", "bf16", 2, 4, 64, [50, 0, 9], [2, 1, 3], prefix=2000, seed=42)
+    target, draft, toks, counts, ua, us = make_verify(T, 43, 6, 4, 50000)
+    drawn, taken = T.zeros(6, 5, dtype=T.int32, device="cuda"), T.zeros(6, dtype=T.int32, device="cuda")
+    pool = Pool(T, q3lib, "e4m3", 40, 4, 128)
+    rows = T.randn(2, 640, 4 * 128, generator=_gen(T, 44), device="cuda")
+    back = T.zeros_like(rows)
+    slots = T.randperm(640, generator=_gen(T, 45), device="cuda").int()
+
+    def verify(stream):
+        q3lib.verify_drafts(drawn.data_ptr(), taken.data_ptr(), target.data_ptr(), target.stride(0),
+                            target.stride(1), draft.data_ptr(), draft.stride(0), draft.stride(1),
+                            toks.data_ptr(), counts.data_ptr(), ua.data_ptr(), us.data_ptr(), 6, 4, 50000,
+                            stream)
+
+    def move(stream):
+        q3lib.kv_write(pool.handle, rows[0].data_ptr(), rows[1].data_ptr(), q3lib.TYPE_F32, 512, 512,
+                       slots.data_ptr(), 640, stream)
+        q3lib.kv_read(pool.handle, back[0].data_ptr(), back[1].data_ptr(), q3lib.TYPE_F32, 512, 512,
+                      slots.data_ptr(), 640, stream)
+
+    calls = [own.call, far.call, verify, move]
+    results = [own.out_buf, far.out_buf, drawn, taken, back]
+    for call in calls:
+        call(None)
+        T.cuda.synchronize()
+    alone = [x.clone() for x in results]
+    own.check()
+    far.check()
+    streams = [T.cuda.Stream() for _ in calls]
+
+    def again():
+        for x in results:
+            x.fill_(9)
+        T.cuda.synchronize()
+
+    again()
+    for _ in range(4):
+        for call, s in zip(calls, streams):
+            call(s.cuda_stream)
+    T.cuda.synchronize()
+    assert all(T.equal(x, y) for x, y in zip(results, alone))
+    main, graph = T.cuda.Stream(), T.cuda.CUDAGraph()
+    with T.cuda.graph(graph, stream=main):
+        for call, s in zip(calls, streams):
+            s.wait_stream(main)
+            call(s.cuda_stream)
+        for s in streams:
+            main.wait_stream(s)
+    again()
+    graph.replay()
+    T.cuda.synchronize()
+    assert all(T.equal(x, y) for x, y in zip(results, alone))
