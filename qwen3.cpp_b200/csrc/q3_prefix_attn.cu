@@ -258,13 +258,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
     auto raw_at = [&](int key, int c) { return key * D + (PANELS == 2 ? c ^ (key & 1) * 4 : c) * 16; };
     const int lw = warp & 3;
     int ids = -1;  // lane: page 2w + (lane & 1) of tile (lane / 2) of the 16 looked up
+    auto look_up_tiles = [&](int j) {
+        const int t = j + lane / 2;
+        const int logical = (tile0 + t) * kPagesPerTile + 2 * lw + (lane & 1);
+        ids = t < n_tiles && logical < all_pages ? __ldg(a.prefix_table + logical) : -1;
+    };
     auto issue = [&](int n, uint8_t* to) {  // in order
         const int j = n >> 1, kind = n & 1;
-        if (!kind && (j & 15) == 0) {
-            const int t = j + lane / 2;
-            const int logical = (tile0 + t) * kPagesPerTile + 2 * lw + (lane & 1);
-            ids = t < n_tiles && logical < all_pages ? __ldg(a.prefix_table + logical) : -1;
-        }
+        if (!kind && (j & 15) == 0 && j > 0) look_up_tiles(j);
         const uint8_t* base = static_cast<const uint8_t*>(kind ? a.v : a.k);
         const int left = a.prefix_len - (tile0 + j) * kKeyTile - lw * 32;  // keys of this warp's 32 that exist
 #pragma unroll
@@ -298,6 +299,29 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
     auto raw = [&](int n) { return sm + L::kRing + n % (L::kRaw ? L::kRaw : 1) * (L::kTile / 2); };
     const int ops = 2 * n_tiles;
     const bool is_loader = warp >= 8 && warp < 12;
+
+    // The CTA's pages and the bytes of their keys: a thread a page. The first of them, and the loaders'
+    // first tiles, are on their way before anything waits.
+    const int n_pages = min(n_tiles * kPagesPerTile, all_pages - tile0 * kPagesPerTile);
+    struct Look {
+        bool in;
+        uint32_t w[E4M3 ? kPageTokens / 2 : 1];
+    };
+    auto look_up = [&](int p, int page) {
+        Look x{};
+        x.in = p < n_pages && page >= 0 && page < a.n_pages;
+        if (E4M3 && x.in) {
+            const uint32_t* e = reinterpret_cast<const uint32_t*>(
+                a.exps + (static_cast<size_t>(page) * a.n_kv + h) * kPageTokens * 2);
+#pragma unroll
+            for (int i = 0; i < kPageTokens / 2; ++i) x.w[E4M3 ? i : 0] = __ldg(e + i);
+        }
+        return x;
+    };
+    auto page_of = [&](int p) { return p < n_pages ? __ldg(a.prefix_table + tile0 * kPagesPerTile + p) : -1; };
+    const int first_page = page_of(tid);
+    if (is_loader) look_up_tiles(0);
+    Look mine = look_up(tid, first_page);
     if (E4M3 && is_loader) {
 #pragma unroll
         for (int n = 0; n < L::kRaw - 1; ++n) {
@@ -331,44 +355,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
         commit();
     }
 
-    // The CTA's pages and the largest bytes of their keys: a thread a page, the first of its pages looked
-    // up before the barriers are ready.
-    const int n_pages = min(n_tiles * kPagesPerTile, all_pages - tile0 * kPagesPerTile);
-    struct Look {
-        bool in;
-        int k, v;
-    };
-    auto look_up = [&](int p) {
-        Look x{false, 0, 0};
-        if (p >= n_pages) return x;
-        const int logical = tile0 * kPagesPerTile + p;
-        const int page = __ldg(a.prefix_table + logical);
-        x.in = page >= 0 && page < a.n_pages;
-        if (E4M3 && x.in) {
-            const uint32_t* e = reinterpret_cast<const uint32_t*>(
-                a.exps + (static_cast<size_t>(page) * a.n_kv + h) * kPageTokens * 2);
-            const int n = min(kPageTokens, a.prefix_len - logical * kPageTokens);
-            uint32_t w[kPageTokens / 2], kt = 0, vt = 0;
-#pragma unroll
-            for (int i = 0; i < kPageTokens / 2; ++i) w[i] = __ldg(e + i);
-#pragma unroll
-            for (int i = 0; i < kPageTokens / 2; ++i) {
-                if (2 * i < n) {
-                    kt = max(kt, w[i] & 0xffu);
-                    vt = max(vt, w[i] >> 8 & 0xffu);
-                }
-                if (2 * i + 1 < n) {
-                    kt = max(kt, w[i] >> 16 & 0xffu);
-                    vt = max(vt, w[i] >> 24);
-                }
-            }
-            x.k = static_cast<int>(kt);
-            x.v = static_cast<int>(vt);
-        }
-        return x;
-    };
-    Look mine = look_up(tid);
-
     if (tid == 0) {
         mbar_init(q_full, PAIR ? 8 : 4);
         for (int i = 0; i < SLOTS; ++i) {
@@ -386,16 +372,33 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
         top_s[0] = top_s[1] = 0;
         mbar_fence_init();
     }
-    for (int i = tid; i < n_tiles; i += kPrefixThreads) mask[i] = 0;
     if (warp == 12) tmem_alloc(tmem_slot, kTmemCols);
     __syncthreads();
-    for (int p = tid; p < n_pages; p += kPrefixThreads) {
-        if (p != tid) mine = look_up(p);
-        if (!mine.in) continue;
-        atomicOr(reinterpret_cast<unsigned*>(mask) + p / 32, 1u << (p % 32));
+    for (int p0 = warp * 32; p0 < n_pages; p0 += kPrefixThreads) {
+        if (p0 != warp * 32) mine = look_up(p0 + lane, page_of(p0 + lane));
+        const unsigned in = __ballot_sync(0xffffffffu, mine.in);
+        if (lane == 0) reinterpret_cast<unsigned*>(mask)[p0 / 32] = in;
         if constexpr (E4M3) {
-            atomicMax(&top_s[0], mine.k);
-            atomicMax(&top_s[1], mine.v);
+            const int n = a.prefix_len - (tile0 * kPagesPerTile + p0 + lane) * kPageTokens;  // the page's keys
+            uint32_t kt = 0, vt = 0;
+#pragma unroll
+            for (int i = 0; i < kPageTokens / 2; ++i) {
+                if (2 * i < n) {
+                    kt = max(kt, mine.w[i] & 0xffu);
+                    vt = max(vt, mine.w[i] >> 8 & 0xffu);
+                }
+                if (2 * i + 1 < n) {
+                    kt = max(kt, mine.w[i] >> 16 & 0xffu);
+                    vt = max(vt, mine.w[i] >> 24);
+                }
+            }
+            // One of 32 lanes: same-address atomics of all would go one after the other.
+            kt = __reduce_max_sync(0xffffffffu, kt);
+            vt = __reduce_max_sync(0xffffffffu, vt);
+            if (lane == 0) {
+                atomicMax(&top_s[0], static_cast<int>(kt));
+                atomicMax(&top_s[1], static_cast<int>(vt));
+            }
         }
     }
     tc_fence_before();
