@@ -65,12 +65,16 @@ constexpr int kInlinePages = 96, kInlineWork = 16384;
 enum Mode { kLine, kStrip, kWideStrip };
 
 // Warps of a block, pages of a warp's ring, and blocks a multiprocessor (registers and rings together).
-template <bool E4M3, int NT, Mode MODE>
+// Heads of 64 leave room for one more: strips of 200 x 4 rows and 100 tokens 28.4 -> 25.8 us, a bf16 pool's
+// line of 40 x 4 rows and 100 to 4000 tokens 26.0 -> 24.6; an e4m3 pool's line is slower for it (64 x 128 to
+// 4096: 40.4 against 36.0).
+template <int D, bool E4M3, int NT, Mode MODE>
 struct Shape {
     static constexpr int kWarps = MODE == kWideStrip ? kStripWarps : q3::kWarps;
     static constexpr int kStages = 2;
     static constexpr int kBlocks = MODE == kWideStrip ? (NT == 1 && E4M3 ? 2 : 1)
-                                                      : (NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2));
+                                                      : (NT == 1 ? (E4M3 ? 4 : 3) : (E4M3 ? 3 : 2)) +
+                                                            (D == 64 && (MODE == kStrip || !E4M3));
 };
 
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from) {
@@ -263,23 +267,23 @@ template <int D, bool E4M3, int NT, Mode MODE>
 struct OwnSmem {
     static constexpr int kRow = E4M3 ? D : 2 * D;                  // bytes of a pool row
     static constexpr int kPage = 2 * kPageTokens * kRow + (E4M3 ? 2 * kPageTokens : 0);  // K, V, bytes
-    static constexpr int kRing = Shape<E4M3, NT, MODE>::kWarps * Shape<E4M3, NT, MODE>::kStages * kPage;
-    static constexpr int kSums = Shape<E4M3, NT, MODE>::kWarps * 8 * NT * D * 4;          // after a run of pages, in its place
+    static constexpr int kRing = Shape<D, E4M3, NT, MODE>::kWarps * Shape<D, E4M3, NT, MODE>::kStages * kPage;
+    static constexpr int kSums = Shape<D, E4M3, NT, MODE>::kWarps * 8 * NT * D * 4;          // after a run of pages, in its place
     static constexpr int kBytes = kRing > kSums ? kRing : kSums;
 };
 
 // kLine: the block takes its run of the line of units. Else it takes one strip and finishes its rows,
 // the prefix's parts among them.
 template <int D, bool E4M3, int NT, Mode MODE>
-__global__ void __launch_bounds__(Shape<E4M3, NT, MODE>::kWarps * 32, Shape<E4M3, NT, MODE>::kBlocks)
+__global__ void __launch_bounds__(Shape<D, E4M3, NT, MODE>::kWarps * 32, Shape<D, E4M3, NT, MODE>::kBlocks)
     own_pages_kernel(const PagedArgs a) {
     constexpr int MT = D / 16;                    // m-tiles of O^T, k-steps of S^T
     constexpr int KW = E4M3 ? D / 16 : D / 8;     // words a lane holds of one K row
     constexpr int VW = E4M3 ? D / 32 : D / 16;    // and of one V row
     using L = OwnSmem<D, E4M3, NT, MODE>;
-    constexpr int W = Shape<E4M3, NT, MODE>::kWarps;
+    constexpr int W = Shape<D, E4M3, NT, MODE>::kWarps;
     constexpr bool LINE = MODE == kLine;
-    constexpr int ROW = L::kRow, PIECES = ROW / 16, STAGES = Shape<E4M3, NT, MODE>::kStages;
+    constexpr int ROW = L::kRow, PIECES = ROW / 16, STAGES = Shape<D, E4M3, NT, MODE>::kStages;
     constexpr int ROWS = 8 * NT;
     extern __shared__ __align__(128) uint8_t ring_s[];
     float (*o_s)[ROWS][D] = reinterpret_cast<float (*)[ROWS][D]>(ring_s);
@@ -857,7 +861,7 @@ void launch_strips(const PagedArgs& a, long long strips, cudaStream_t s) {
     auto kernel = own_pages_kernel<D, E4M3, NT, MODE>;
     Q3_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     launch_dep(a.prefix_splits > 0, kernel, dim3(static_cast<unsigned>(strips)),
-               dim3(Shape<E4M3, NT, MODE>::kWarps * 32), bytes, s, a);
+               dim3(Shape<D, E4M3, NT, MODE>::kWarps * 32), bytes, s, a);
 }
 
 template <int D, bool E4M3, int NT>
@@ -870,7 +874,7 @@ void launch_own(const PagedArgs& a, int sms, cudaStream_t s) {
         else launch_strips<D, E4M3, NT, kStrip>(a, strips, s);
         return;
     }
-    constexpr int per_sm = Shape<E4M3, NT, kLine>::kBlocks, bytes = OwnSmem<D, E4M3, NT, kLine>::kBytes;
+    constexpr int per_sm = Shape<D, E4M3, NT, kLine>::kBlocks, bytes = OwnSmem<D, E4M3, NT, kLine>::kBytes;
     // No more blocks than the table's width could fill.
     const long long most = (strips * (a.table_stride + kSetup) + kMinUnits - 1) / kMinUnits;
     const int grid = static_cast<int>(
