@@ -27,9 +27,9 @@
 // CTA's loops and leaves NaN in its parts.
 //
 // Bound by 4 * D operations a row, head and key for many rows, by latency for few. 427 rows of 32 heads,
-// 8 KV heads of 128, 32768 keys (e4m3): 229 GFLOP in 264 us alone, 0.87 PFLOP/s, the tensor pipe and the
+// 8 KV heads of 128, 32768 keys (e4m3): 229 GFLOP in 267 us alone, 0.86 PFLOP/s, the tensor pipe and the
 // exponentials' 41% busy each, shared memory about 68% (scores read 128 bytes a cycle, the loaders write
-// the raw and the converted tiles), the power limit reached. 8192 keys for 64 rows of 16 heads: 18 us.
+// the raw and the converted tiles), the power limit reached. 8192 keys for 64 rows of 16 heads: 16 us.
 #include <algorithm>
 
 #include "q3_paged_attn.cuh"
