@@ -300,8 +300,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
     const int ops = 2 * n_tiles;
     const bool is_loader = warp >= 8 && warp < 12;
 
-    // The CTA's pages and the bytes of their keys: a thread a page. The first of them, and the loaders'
-    // first tiles, are on their way before anything waits.
+    // The CTA's pages and the bytes of their keys: a thread a page. The first are on their way before anything
+    // waits, the loaders' behind their first tiles (64 x 8192: 32.5 us, 33.4 with all of them after the set-up).
     const int n_pages = min(n_tiles * kPagesPerTile, all_pages - tile0 * kPagesPerTile);
     struct Look {
         bool in;
@@ -321,13 +321,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
     auto page_of = [&](int p) { return p < n_pages ? __ldg(a.prefix_table + tile0 * kPagesPerTile + p) : -1; };
     const int first_page = page_of(tid);
     if (is_loader) look_up_tiles(0);
-    Look mine = look_up(tid, first_page);
+    Look mine{};
+    if (!E4M3 || !is_loader) mine = look_up(tid, first_page);
     if (E4M3 && is_loader) {
 #pragma unroll
         for (int n = 0; n < L::kRaw - 1; ++n) {
             if (n < ops) issue(n, raw(n));
             commit();
         }
+        mine = look_up(tid, first_page);
     }
     // ---------------------------------------------------------------- softmax: the rows of Q on their way
     // Whole rows, Q_LANES lanes each, into their places in the operand (a thread reading its own row from
