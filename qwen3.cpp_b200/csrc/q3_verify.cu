@@ -18,6 +18,7 @@
 #include <climits>
 
 #include "q3_paged.cuh"
+#include "q3_verify_pieces.cuh"
 
 namespace q3 {
 
@@ -36,11 +37,8 @@ struct VerifyArgs {
     int max_drafts, vocab, ctas;  // ctas: of a sequence's cluster
 };
 
-constexpr int kVerifyThreads = 512;   // at most
 constexpr int kVerifyWarps = kVerifyThreads / 32;
-constexpr int kUnroll = 2;           // 16-byte loads of p, and of q, that a lane has on their way (5: 6% slower)
-constexpr int kMaxCtas = 16;       // of a cluster
-constexpr int kLeastShare = 4096;  // values that are worth a CTA: below, its start costs more than it reads
+constexpr int kUnroll = 2;  // 16-byte loads of p, and of q, that a lane has on their way (5: 6% slower)
 
 __device__ __forceinline__ float share(float x) { return x > 0.0f ? x : 0.0f; }  // NaN is 0
 
@@ -139,8 +137,6 @@ __device__ __forceinline__ double running_sum(double x) {
     return x;
 }
 
-constexpr int kScan = 128;  // values that one warp scans
-
 // First index of [i0, i1), at most kScan values, at which the running sum, `before` in front of it,
 // passes goal; `last` if the roundings of another order keep it from that.
 template <int V>
@@ -200,18 +196,17 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     row.p = a.target + b * a.t_seq + n * a.t_row;
     row.q = n < count && a.draft ? a.draft + b * a.d_seq + n * a.d_row : nullptr;
     row.one = n < count && !a.draft ? tok[n] : -1;
-    // Pieces start on multiples of 4, so that they are as aligned as the row.
-    const long long pieces = static_cast<long long>(a.ctas) * n_warps;
-    const int per = static_cast<int>(((a.vocab + pieces - 1) / pieces + 3) / 4 * 4);
-    const int i0 = static_cast<int>(min(static_cast<long long>(a.vocab), (rank * n_warps + warp) * static_cast<long long>(per)));
-    const int i1 = static_cast<int>(min(static_cast<long long>(a.vocab), i0 + static_cast<long long>(per)));
+    // This CTA's share of the row, the same in all its threads, and this warp's piece of it.
+    const int per = piece_step(a.vocab, a.ctas * n_warps);
+    const Span cta = piece({0, a.vocab}, static_cast<long long>(per) * n_warps, rank);
+    const Span own = piece(cta, per, warp);
     const bool vec = ((reinterpret_cast<uintptr_t>(row.p) | reinterpret_cast<uintptr_t>(row.q)) & 15) == 0;
     // The sums before this CTA's share and up to its end, added up in one order everywhere, so that one's
     // end is the next one's beginning to the bit and every goal lies in exactly one.
     double total = 0.0, cta_before = 0.0, cta_after = 0.0;
     int last = -1;
     for (int attempt = 0; attempt < 2; ++attempt) {
-        const Piece mine = vec ? sum_piece<4, kUnroll>(row, i0, i1) : sum_piece<1, kUnroll>(row, i0, i1);
+        const Piece mine = vec ? sum_piece<4, kUnroll>(row, own.i0, own.i1) : sum_piece<1, kUnroll>(row, own.i0, own.i1);
         if (lane == 0) warps_s[warp] = mine;
         if (attempt == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         __syncthreads();
@@ -249,13 +244,14 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
     int32_t* out = a.tokens + static_cast<size_t>(b) * (a.max_drafts + 1);
     if (cta_before <= goal && goal < cta_after) {
         // The token lies in this CTA's share: its warps cut the warp's piece it lies in among them until
-        // one warp can scan what is left (one round for 1e5 values).
-        int j0 = i0 - warp * per, j1 = static_cast<int>(min(static_cast<long long>(a.vocab), j0 + static_cast<long long>(per) * n_warps));
+        // one warp can scan what is left (one round for 1e5 values). The span that is cut is the same in every
+        // thread, so all leave in the same round.
+        Span span = cta;
         int step = per;
         double base = cta_before;
         int at = -1;
         while (true) {
-            // The piece among [j0, j1)'s that the goal lies in; the last with a share if roundings put it
+            // The piece among the span's that the goal lies in; the last with a share if roundings put it
             // behind all of them. Every warp works it out, a lane a piece.
             Piece x{0.0, -1};
             if (lane < n_warps) x = warps_s[lane];
@@ -265,16 +261,18 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyA
             const int pick = past ? __ffs(past) - 1 : 31 - __clz(has | 1u);
             const int pick_last = __shfl_sync(0xffffffffu, x.last, pick);
             const double below = __shfl_sync(0xffffffffu, base + (up_to - x.sum), pick);
-            j0 += pick * step;
-            j1 = min(j1, j0 + step);
+            span = piece(span, step, pick);
             base = below;
-            if (j1 - j0 <= kScan) {
-                if (warp == 0) at = vec ? scan<4>(row, j0, j1, base, goal, pick_last) : scan<1>(row, j0, j1, base, goal, pick_last);
+            if (span.size() <= kScan) {
+                if (warp == 0) {
+                    at = vec ? scan<4>(row, span.i0, span.i1, base, goal, pick_last)
+                             : scan<1>(row, span.i0, span.i1, base, goal, pick_last);
+                }
                 break;
             }
-            step = ((j1 - j0 + n_warps - 1) / n_warps + 3) / 4 * 4;
-            const int k0 = min(j1, j0 + warp * step), k1 = min(j1, k0 + step);
-            const Piece mine = vec ? sum_piece<4, 1>(row, k0, k1) : sum_piece<1, 4>(row, k0, k1);
+            step = piece_step(span.size(), n_warps);
+            const Span sub = piece(span, step, warp);
+            const Piece mine = vec ? sum_piece<4, 1>(row, sub.i0, sub.i1) : sum_piece<1, 4>(row, sub.i0, sub.i1);
             __syncthreads();
             if (lane == 0) warps_s[warp] = mine;
             __syncthreads();
@@ -323,12 +321,7 @@ extern "C" q3_status q3_verify_drafts(int32_t* tokens, int32_t* n_accepted, cons
         }
         const q3::OnDevice on({tokens, n_accepted, target, draft, max_drafts ? draft_tokens : nullptr,
                                n_drafts, max_drafts ? u_accept : nullptr, u_sample});
-        // As many CTAs as have kLeastShare values each, a power of two: up to 16 for up to 4 sequences (a
-        // multiprocessor reads about 40 GB/s from L2, so one sequence's row takes 7.1 us on 16 and 8.3
-        // on 8), else up to 8 (clusters of 16 find room less easily: 64 sequences 36 us against 24).
-        const int most = n_seqs <= 4 ? q3::kMaxCtas : q3::kMaxCtas / 2;
-        int ctas = 1;
-        while (ctas < most && vocab >= 2 * ctas * q3::kLeastShare) ctas *= 2;
+        const int ctas = q3::verify_ctas(n_seqs, vocab);
         if (n_seqs > INT_MAX / ctas) throw std::invalid_argument("draft verification: size out of range");
         const q3::VerifyArgs a{tokens, n_accepted, target, draft, draft_tokens, n_drafts, u_accept,
                                u_sample, t_seq, t_row, d_seq, d_row, max_drafts, vocab, ctas};
@@ -337,10 +330,7 @@ extern "C" q3_status q3_verify_drafts(int32_t* tokens, int32_t* n_accepted, cons
         }
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(n_seqs) * ctas);
-        // With more CTAs than multiprocessors, smaller ones, so that they are all resident at once (64
-        // sequences: 24 us against 28); else the larger, whose lanes go round less often.
-        cfg.blockDim = dim3(static_cast<long long>(n_seqs) * ctas > on.sm_count() ? q3::kVerifyThreads / 2
-                                                                                 : q3::kVerifyThreads);
+        cfg.blockDim = dim3(static_cast<unsigned>(q3::verify_threads(n_seqs, ctas, on.sm_count())));
         cfg.stream = static_cast<cudaStream_t>(stream);
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
