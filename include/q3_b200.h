@@ -417,7 +417,9 @@ q3_status q3_kv_read(const q3_kv_pool* pool, void* k, void* v, int type, int64_t
  * (either pool) or F16 (an e4m3 pool), 16-byte aligned; n_heads a multiple of pool->n_kv_heads, at
  * most 64 query heads per KV head; scores are divided by sqrt(head_dim). max_q * n_heads /
  * n_kv_heads is at most 128. workspace: q3_paged_attn_workspace_size bytes (prefix_len 0), 16-byte
- * aligned, used by one call at a time. Sums and softmax statistics are fp32; the probabilities are
+ * aligned, used by one call at a time. The size never falls as n_q, n_seqs, max_q or prefix_len grow:
+ * one that was allocated for the largest of each serves every smaller call. (0 for sizes that the calls
+ * refuse.) Sums and softmax statistics are fp32; the probabilities are
  * rounded to fp16 for an e4m3 pool, split into two bf16 values for a bf16 one. */
 size_t q3_paged_attn_workspace_size(const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs,
                                     int max_q, int prefix_len);

@@ -906,15 +906,20 @@ bool sizes_ok(const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs, int max_
            static_cast<long long>(n_seqs) * max_q * n_heads <= INT_MAX;
 }
 
-// Lays the workspace out from its start; returns its size.
-size_t lay_out(PagedArgs& a, uint8_t* base, int head_dim) {
-    size_t at = 0;
+// Rows of a strip.
+int strip_rows(const PagedArgs& a) { return a.max_q * a.group <= 8 ? 8 : 16; }
+
+// The workspace's arrays begin on multiples of 256 bytes.
+size_t whole_lines(size_t bytes) { return (bytes + 255) & ~size_t(255); }
+
+// Lays the workspace out from its start for this call.
+void lay_out(PagedArgs& a, uint8_t* base, int head_dim) {
     auto take = [&](size_t bytes) {
-        uint8_t* p = base + at;
-        at += (bytes + 255) & ~size_t(255);
+        uint8_t* p = base;
+        base += whole_lines(bytes);
         return p;
     };
-    const size_t rows = a.max_q * a.group <= 8 ? 8 : 16;
+    const size_t rows = strip_rows(a);
     a.own_ml = reinterpret_cast<float2*>(take(kMaxBlocks * 2 * rows * 8));
     a.own_o = reinterpret_cast<float*>(take(kMaxBlocks * 2 * rows * head_dim * 4));
     if (a.prefix_len > 0) {
@@ -925,6 +930,17 @@ size_t lay_out(PagedArgs& a, uint8_t* base, int head_dim) {
         a.prefix_splits = prefix_splits(a.n_kv, a.prefix_rows, a.prefix_len);
         a.prefix_ml = reinterpret_cast<float2*>(take(a.prefix_splits * all * 8));
         a.prefix_o = reinterpret_cast<float*>(take(a.prefix_splits * all * head_dim * 4));
+    }
+}
+
+// The size that the call, and every call of fewer rows, sequences, rows a sequence or shared tokens, lays out.
+size_t workspace_size(const PagedArgs& a, int head_dim) {
+    const size_t cell = static_cast<size_t>(head_dim) * 4, rows = strip_rows(a);
+    size_t at = whole_lines(kMaxBlocks * 2 * rows * 8) + whole_lines(kMaxBlocks * 2 * rows * cell);
+    if (a.prefix_len > 0) {
+        const size_t all = static_cast<size_t>(a.n_kv) * a.n_q * a.group;
+        const size_t parts = a.n_kv * prefix_part_rows(a.n_kv, a.n_q * a.group, a.prefix_len);
+        at += whole_lines(all * 8) + whole_lines(all * cell) + whole_lines(parts * 8) + whole_lines(parts * cell);
     }
     return at;
 }
@@ -981,8 +997,8 @@ void paged_attention(void* out, void* workspace, const void* q, int type, int64_
     lay_out(a, static_cast<uint8_t*>(workspace), pool->head_dim);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool e4m3 = pool->type == Q3_TYPE_E4M3;
-    const int strip_rows = max_q * a.group <= 8 ? 8 : 16;
-    const long long strips = static_cast<long long>(n_seqs) * a.n_kv * ((max_q * a.group + strip_rows - 1) / strip_rows);
+    const int rows = strip_rows(a);
+    const long long strips = static_cast<long long>(n_seqs) * a.n_kv * ((max_q * a.group + rows - 1) / rows);
     const long long pages = (prefix_len + kPageTokens - 1LL) / kPageTokens;
     if (pages + table_stride <= kInlinePages && strips * pages <= kInlineWork) {
         a.inline_pages = static_cast<int>(pages);
@@ -1016,7 +1032,7 @@ size_t q3_paged_attn_workspace_size(const q3_kv_pool* pool, int n_heads, int n_q
     a.n_seqs = n_seqs;
     a.max_q = max_q;
     a.prefix_len = prefix_len;
-    return q3::lay_out(a, nullptr, pool->head_dim);
+    return q3::workspace_size(a, pool->head_dim);
 }
 
 q3_status q3_paged_attn(void* out, void* workspace, const void* q, int type, int64_t q_stride,

@@ -88,5 +88,8 @@ __device__ __forceinline__ uint32_t pack2_out(float lo, float hi, int f16) {
 void launch_prefix_attention(const PagedArgs& a, int head_dim, bool e4m3, cudaStream_t s);
 // Parts that the prefix kernel leaves for each row, from the sizes alone.
 int prefix_splits(int n_kv, int rows, int prefix_len);
+// The most parts, of all rows together, that a batch of so many rows or fewer leaves over a prefix of this
+// length or a shorter one.
+size_t prefix_part_rows(int n_kv, int rows, int prefix_len);
 
 }  // namespace q3

@@ -787,23 +787,64 @@ void launch(const PagedArgs& a, bool e4m3, cudaStream_t s) {
 
 // Parts per row. A CTA's time is about (its key tiles + 3), 3 for its start and end (with 5, 8 or 12 the
 // same splits come out at 32768 keys, with 1 others that are 16% slower); the splits make the sum over the
-// waves of 148 CTAs least.
+// waves of 148 CTAs least. They do not ask the device, as the workspace's size has to know them too.
+//
+// The workspace of a batch has to serve every smaller one, but the best splits jump both ways with the number
+// of tiles. So they are sought up to most_splits, the best for tiles that could be cut anywhere: for that the
+// time is waves(n) * tiles / n + 3 * waves(n), a line over the tiles for each n, flatter and higher for more
+// splits, so the least of the lines moves to more splits as tiles grow and never back. (Fewer than 1 choice in
+// 100 changes by that, 7% of the time at worst by this count.)
+namespace {
+
+struct Cut {
+    long long base, tiles, least, most;  // CTAs of one split, key tiles, and splits that are possible
+    bool pair;
+    Cut(int n_kv, long long rows, int prefix_len) : pair(rows > kRowTile) {
+        base = static_cast<long long>(n_kv) * (pair ? (rows + 2 * kRowTile - 1) / (2 * kRowTile) : 1);
+        tiles = (static_cast<long long>(prefix_len) + kKeyTile - 1) / kKeyTile;
+        least = (tiles + kMaxTiles - 1) / kMaxTiles;
+        most = std::max(least, std::min(tiles, 64LL));
+    }
+    long long waves(long long n) const { return (base * n + 147) / 148; }
+    long long most_splits() const {
+        long long best = least, best_time = -1;
+        for (long long n = least; n <= most; ++n) {
+            const long long time = waves(n) * ((pair ? 2 : 1) * tiles + 3 * n);  // n times it
+            if (best_time < 0 || time * best <= best_time * n) {
+                best = n;
+                best_time = time;
+            }
+        }
+        return best;
+    }
+};
+
+}  // namespace
+
 int prefix_splits(int n_kv, int rows, int prefix_len) {
     if (prefix_len <= 0 || rows <= 0) return 0;
-    const bool pair = rows > kRowTile;
-    const long long base = static_cast<long long>(n_kv) * (pair ? (rows + 2 * kRowTile - 1) / (2 * kRowTile) : 1);
-    const long long tiles = (static_cast<long long>(prefix_len) + kKeyTile - 1) / kKeyTile;
-    const long long least = (tiles + kMaxTiles - 1) / kMaxTiles;
-    long long best = least, best_cost = -1;
-    for (long long n = least; n <= std::max(least, std::min(tiles, 64LL)); ++n) {
-        const long long waves = (base * n + 147) / 148, each = (tiles + n - 1) / n;
-        const long long cost = waves * ((pair ? 2 : 1) * each + 3);
-        if (best_cost < 0 || cost < best_cost) {
+    const Cut cut(n_kv, rows, prefix_len);
+    const long long most = cut.most_splits();
+    long long best = cut.least, best_time = -1;
+    for (long long n = cut.least; n <= most; ++n) {
+        const long long each = (cut.tiles + n - 1) / n, time = cut.waves(n) * ((cut.pair ? 2 : 1) * each + 3);
+        if (best_time < 0 || time < best_time) {
             best = n;
-            best_cost = cost;
+            best_time = time;
         }
     }
     return static_cast<int>(best);
+}
+
+size_t prefix_part_rows(int n_kv, int rows, int prefix_len) {
+    if (prefix_len <= 0 || rows <= 0) return 0;
+    // The most rows of each number of row tiles: one tile alone, then pairs.
+    long long most = std::min(rows, kRowTile) * Cut(n_kv, 1, prefix_len).most_splits();
+    for (long long n = 2 * kRowTile; rows > kRowTile; n += 2 * kRowTile) {
+        most = std::max(most, std::min<long long>(rows, n) * Cut(n_kv, n, prefix_len).most_splits());
+        if (n >= rows) break;
+    }
+    return static_cast<size_t>(most);
 }
 
 void launch_prefix_attention(const PagedArgs& a, int head_dim, bool e4m3, cudaStream_t s) {
