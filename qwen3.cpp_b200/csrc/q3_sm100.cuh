@@ -65,11 +65,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, long lon
 }
 // mbar_wait for every lane of a converged warp: a non-blocking probe by every lane first, so a
 // phase that has already completed costs one probe (a blocking try_wait by 32 lanes costs
-// hundreds of cycles even then).
+// hundreds of cycles even then). All lanes get the same answer: each keeps its own time and sees *abort for
+// itself, so where some give up and others do not, the warp gives up, and goes on together.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* b, uint32_t parity, long long budget,
                                                volatile int* abort) {
     if (__all_sync(0xffffffffu, mbar_test_wait(b, parity))) return true;
-    return mbar_wait(b, parity, budget, abort);
+    return __all_sync(0xffffffffu, mbar_wait(b, parity, budget, abort));
 }
 
 // 2-D tiled TMA load global -> shared (this CTA), completing on an mbarrier. x is the innermost
