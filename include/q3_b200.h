@@ -420,7 +420,9 @@ q3_status q3_kv_read(const q3_kv_pool* pool, void* k, void* v, int type, int64_t
  * aligned, used by one call at a time. The size never falls as n_q, n_seqs, max_q or prefix_len grow:
  * one that was allocated for the largest of each serves every smaller call. (0 for sizes that the calls
  * refuse.) Sums and softmax statistics are fp32; the probabilities are
- * rounded to fp16 for an e4m3 pool, split into two bf16 values for a bf16 one. */
+ * rounded to fp16 for an e4m3 pool, split into two bf16 values for a bf16 one (2^-16). An infinite
+ * value of a bf16 pool makes that place of the rows that see it this infinity (NaN where both meet, or
+ * where the token's weight is below about 2^-118 of the row's largest). */
 size_t q3_paged_attn_workspace_size(const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs,
                                     int max_q, int prefix_len);
 q3_status q3_paged_attn(void* out, void* workspace, const void* q, int type, int64_t q_stride,

@@ -608,9 +608,9 @@ __global__ void __launch_bounds__(Shape<D, E4M3, NT, MODE>::kWarps * 32, Shape<D
                         const float f = tail && g + 8 * x >= limit ? 0.0f : vf[x];
                         pb[n][x] = transpose8x8(pack2_out(lo * f, hi * f, 1));
                     } else {
-                        const uint32_t w = pack2_bf16(lo, hi);
+                        const uint32_t w = weights_hi(lo, hi);
                         pb[n][x] = transpose8x8(w);
-                        pl[n][x] = transpose8x8(pack2_bf16(lo - bf16_lo(w), hi - bf16_hi(w)));
+                        pl[n][x] = transpose8x8(weights_lo(lo, hi, w));
                     }
                 }
             }

@@ -77,6 +77,16 @@ __device__ __forceinline__ uint32_t pack2_bf16(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// Two weights as hi + lo in bf16, for a bf16 pool. hi is the weight cut off, and lo the rest with 2^-23 of the
+// weight on top, rounded (2^-16 of the weight): both are positive where the weight is, so that an infinite value
+// times them is that infinity. (A rounded hi leaves a lo of zero or less for half of the weights, and NaN.)
+__device__ __forceinline__ uint32_t weights_hi(float x, float y) {
+    return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632u);
+}
+__device__ __forceinline__ uint32_t weights_lo(float x, float y, uint32_t hi) {
+    constexpr float kOnTop = 1.00000011920928955078125f;  // 1 + 2^-23
+    return pack2_bf16(fmaf(x, kOnTop, -bf16_lo(hi)), fmaf(y, kOnTop, -bf16_hi(hi)));
+}
 // Two results in the caller's type, to nearest even; an fp16 result past the range becomes infinity.
 __device__ __forceinline__ uint32_t pack2_out(float lo, float hi, int f16) {
     if (!f16) return pack2_bf16(lo, hi);

@@ -675,14 +675,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                     p.y = ex2(p.y);
                     x[half * 64 + k] = p.x;
                     x[half * 64 + k + 1] = p.y;
-                    y[k / 2] = E4M3 ? pack2_out(p.x, p.y, 1) : pack2_bf16(p.x, p.y);
+                    y[k / 2] = E4M3 ? pack2_out(p.x, p.y, 1) : weights_hi(p.x, p.y);
                 }
                 tmem_st32(s_at + half * 32, y);
                 if constexpr (!E4M3) {
                     uint32_t lo[32];
 #pragma unroll
                     for (int k = 0; k < 64; k += 2) {
-                        lo[k / 2] = pack2_bf16(x[half * 64 + k] - bf16_lo(y[k / 2]), x[half * 64 + k + 1] - bf16_hi(y[k / 2]));
+                        lo[k / 2] = weights_lo(x[half * 64 + k], x[half * 64 + k + 1], y[k / 2]);
                     }
                     tmem_st32(s_at + 64 + half * 32, lo);
                 }

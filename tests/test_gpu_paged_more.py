@@ -19,3 +19,56 @@ def test_a_larger_batchs_workspace(T, q3lib, large, small):  # noqa: F811
     b.call()
     b.check()
     assert bool((b.ws[size:] == 0xFF).all())
+
+
+def _set_value(pool, slot, d, x):
+    """Value d of every KV head of a bf16 pool's V row, or the code byte of an e4m3 one's."""
+    pool.v[slot // 16, :, slot % 16, d] = x
+
+
+@pytest.mark.parametrize("h,group,d", [(2, 2, 128), (3, 5, 64), (1, 16, 128)])
+@pytest.mark.parametrize("own,width,prefix,at", [
+    ([40, 33], None, 0, "last"), ([40, 33], None, 0, "first"),        # a block a strip
+    ([1300, 700], 90, 0, "last"), ([1300, 700], 90, 0, "first"),      # the line, cut among blocks
+    ([40, 33], None, 300, "prefix"),                                  # a prefix in the strips
+    ([40, 33], 100, 300, "prefix"), ([3, 700], 100, 2000, "prefix"),  # on the tensor cores, one row tile
+])
+def test_infinite_values_of_a_bf16_pool(T, q3lib, h, group, d, own, width, prefix, at):  # noqa: F811
+    """+infinity and -infinity among a token's values are the results of the rows that see it, in those places
+    alone; whatever the weights' low halves are. (Scores are small, so that no weight underflows.)"""
+    b = Batch(T, q3lib, "bf16", "bf16", h, group, d, own, [3, 2], prefix=prefix, seed=61, q_scale=0.25)
+    if width:
+        b.widen(width)
+    # "last": of the first sequence's newest token, seen by its last row alone.
+    slot = int({"last": b.slots[0][-1], "first": b.slots[0][0],
+                "prefix": b.prefix_slots[-20] if prefix else -1}[at])
+    sees = {"last": [2], "first": [0, 1, 2], "prefix": [0, 1, 2, 3, 4]}[at]
+    for place in (5, 40):
+        _set_value(b.pool, slot, place, 0.0)
+    val, err = b.want()
+    _set_value(b.pool, slot, 5, math.inf)
+    _set_value(b.pool, slot, 40, -math.inf)
+    b.call()
+    T.cuda.synchronize()
+    got = b.out_buf[:5].double().view(5, h * group, d)
+    want = val[:5].clone()
+    want[sees, :, 5], want[sees, :, 40] = math.inf, -math.inf
+    there = want.isfinite()
+    assert bool((got[~there] == want[~there]).all())
+    assert bool((got - want)[there].abs().le(err[:5][there]).all())
+
+
+def test_infinite_values_of_many_rows(T, q3lib):  # noqa: F811
+    """The same over a prefix for the rows of several tiles."""
+    b = Batch(T, q3lib, "bf16", "bf16", 2, 4, 128, [5 + i % 40 for i in range(90)], [1] * 90, prefix=2500, seed=62,
+              q_scale=0.25)
+    slot = int(b.prefix_slots[777])
+    _set_value(b.pool, slot, 5, 0.0)
+    val, err = b.want()
+    _set_value(b.pool, slot, 5, math.inf)
+    b.call()
+    T.cuda.synchronize()
+    got = b.out_buf[:90].double().view(90, 8, 128)
+    assert bool((got[:, :, 5] == math.inf).all())
+    rest = [i for i in range(128) if i != 5]
+    assert bool((got - val[:90]).abs().le(err[:90])[:, :, rest].all())
