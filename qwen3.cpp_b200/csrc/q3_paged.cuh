@@ -89,7 +89,7 @@ inline void check_pool(const q3_kv_pool* pool) {
 
 // 2^(byte - 127); a float's exponent field, but for byte 0 (2^-127 is subnormal).
 __device__ __forceinline__ float exp_of_byte(uint32_t byte) {
-    return __uint_as_float(byte ? byte << 23 : 0x00400000u);
+    return __uint_as_float(max(byte << 23, 0x00400000u));
 }
 
 // Two e4m3 codes (the low 16 bits of `pair`) as packed fp16: every e4m3 value is an fp16 value.

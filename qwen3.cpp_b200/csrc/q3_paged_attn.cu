@@ -521,13 +521,14 @@ __global__ void __launch_bounds__(Shape<D, E4M3, NT, MODE>::kWarps * 32, Shape<D
             }
             const bool tail = !there || key0 + kPageTokens > (shared ? a.prefix_len : tail_key);
             const int limit = there ? (shared ? a.prefix_len : s.len) - key0 : 0;  // this page's keys that exist
+            const float k_factor[2] = {exp_of_byte(ex[0] & 0xffu), exp_of_byte(ex[1] & 0xffu)};
             float p[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     p[n][i] = sc[n][i] * (E4M3 ? c_col[n][i & 1] : c_col[0][0]);
-                    if constexpr (E4M3) p[n][i] *= __uint_as_float((ex[i >> 1] & 0xffu) << 23);  // 2^(byte - 127)
+                    if constexpr (E4M3) p[n][i] *= k_factor[i >> 1];
                 }
             }
             if (tail) {

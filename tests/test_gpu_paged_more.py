@@ -72,3 +72,26 @@ def test_infinite_values_of_many_rows(T, q3lib):  # noqa: F811
     assert bool((got[:, :, 5] == math.inf).all())
     rest = [i for i in range(128) if i != 5]
     assert bool((got - val[:90]).abs().le(err[:90])[:, :, rest].all())
+
+
+@pytest.mark.parametrize("own,width,prefix", [([40, 33], None, 0), ([1300, 700], 90, 0), ([40, 33], None, 300),
+                                              ([40, 33], 100, 300)])
+def test_byte_zero_is_a_power_of_two(T, q3lib, own, width, prefix):  # noqa: F811
+    """A row of byte 0 has the values code * 2^-127, also for queries that make scores of it: all queries are
+    +-2^115, one key has the code 448 with their signs (score 448 * 128 * 2^-12 / sqrt(128) = 1.24), the others
+    are zeros (byte 0 too)."""
+    b = Batch(T, q3lib, "e4m3", "bf16", 1, 1, 128, own, [1, 1], prefix=prefix, seed=63, spare_rows=0)
+    if width:
+        b.widen(width)
+    b.q_buf.copy_(T.where(b.q_buf > 0, 2.0 ** 115, -2.0 ** 115))
+    b.q_buf[1] = b.q_buf[0]
+    for s in b.slots + [b.prefix_slots]:
+        if len(s):
+            v = b.pool.get("v", s)
+            b.pool.put(s, T.zeros_like(v), v)
+    slot = b.prefix_slots[7:8] if prefix else b.slots[0][7:8]
+    v = b.pool.get("v", slot) + 300.0
+    b.pool.put(slot, (448 * 2.0 ** -127 * b.q_buf[0].double().sign()).view(1, 1, 128), v)
+    assert int(b.pool.exps[int(slot) // 16, 0, int(slot) % 16, 0]) == 0
+    b.call()
+    b.check()
