@@ -419,10 +419,13 @@ q3_status q3_kv_read(const q3_kv_pool* pool, void* k, void* v, int type, int64_t
  * n_kv_heads is at most 128. workspace: q3_paged_attn_workspace_size bytes (prefix_len 0), 16-byte
  * aligned, used by one call at a time. The size never falls as n_q, n_seqs, max_q or prefix_len grow:
  * one that was allocated for the largest of each serves every smaller call. (0 for sizes that the calls
- * refuse.) Sums and softmax statistics are fp32; the probabilities are
- * rounded to fp16 for an e4m3 pool, split into two bf16 values for a bf16 one (2^-16). An infinite
- * value of a bf16 pool makes that place of the rows that see it this infinity (NaN where both meet, or
- * where the token's weight is below about 2^-118 of the row's largest). */
+ * refuse.)
+ * Sums and softmax statistics are fp32. For an e4m3 pool query rows become fp16 relative to a power of two
+ * (exact down to 2^-27 of the row's largest value), and the probabilities times their V rows' powers of two are
+ * rounded to fp16 (2^-11; below 2^-21 of the row's largest such product to 2^-32 of it). Queries of 2^113 and
+ * more can leave fp32's range before a small K row brings their score back. For a bf16 pool the probabilities
+ * are split into two bf16 values (2^-16), and an infinite value makes that place of the rows that see it this
+ * infinity (NaN where both meet, or where the token's weight is below about 2^-118 of the row's largest). */
 size_t q3_paged_attn_workspace_size(const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs,
                                     int max_q, int prefix_len);
 q3_status q3_paged_attn(void* out, void* workspace, const void* q, int type, int64_t q_stride,

@@ -25,13 +25,17 @@
 // instead of 37.1). 16-byte piece c of row r lies at piece c ^ (r % 8), which leaves the operand reads
 // without bank conflicts.
 //
-// The running maximum moves only when a score passes it by more than 2^4 (one vote a page instead of
-// two times three shuffles): weights are then at most 2^(kShift + 4), which fp16 holds, as it does 2^3
-// more for V rows' own powers of two, whose running maximum is treated alike.
+// A row's running maximum moves only when a weight passes it by more than 2^4 (bf16 pool; one vote a page
+// instead of two times three shuffles). In an e4m3 pool the weight that meets V is p times the power of two
+// of the V row, which fp16 has to hold: the maximum is that of these products over the keys that the row sees,
+// moved when one passes it by more than 2^7. What fp16 cuts off is then 2^-32 of the row's largest weighted
+// V row, whatever rows hold that have no weight or that later rows alone see. The sum of p, in fp32, has room
+// for p of 2^64 before its own reference moves. References are whole powers of two.
 //
 // Rounding: e4m3 -> fp16 is exact; a query row is scaled by a power of two so that its largest value
 // is in [2^13, 2^14): bf16 and fp16 values are then fp16 values down to 2^-38 of the row's largest.
-// Weights are rounded to fp16 (2^-11), for a bf16 pool to a bf16 pair hi + lo (2^-16). Sums are fp32.
+// Weights, with V's power of two, are rounded to fp16 (2^-11), for a bf16 pool to a bf16 pair hi + lo (2^-16).
+// Sums are fp32.
 //
 // Bound by HBM: 2 * (D + 1) bytes a key and KV head (e4m3). 64 sequences of 128 to 4096 tokens, 8 KV heads
 // of 128: 279 MB in 53.5 us, 5.2 TB/s with the start, the last blocks and the join, about 6 TB/s between
@@ -48,8 +52,9 @@ namespace {
 constexpr int kWarps = 4;                // of a block on the line, and of the join
 constexpr int kThreads = kWarps * 32;
 constexpr int kStripWarps = 8;           // of a strip's block where there are few strips
-constexpr float kGrow = 4.0f;  // how far (log2) a score may pass the running maximum
-constexpr int kGrowV = 3;      // the same for V's powers of two
+// log2 of the largest p, and of the largest p times V's power of two, that leave their references where they are.
+constexpr float kTopBf16 = kShift + 4.0f, kTopE4m3 = 64.0f, kTopV = 15.0f;
+constexpr float kUnseen = 1e38f;  // reference of a row that has seen no key: any score then passes the top
 
 // Tables of up to so many pages take a block a strip: 1 sequence of 512 tokens 7.2 us against 8.4 with
 // the line, whose scan and join cost about 4 us.
@@ -460,14 +465,15 @@ __global__ void __launch_bounds__(Shape<D, E4M3, NT, MODE>::kWarps * 32, Shape<D
         }
         const int tail_key = s.len - s.rows + token_of(a, r_base) + 1;  // seen by every row below it
 
-        float m[NT][2], lim[NT][2], neg[NT][2], l[NT][2], o[NT][MT][4];  // lim = m + kGrow, neg = kShift - m
-        int r_v = -1000;  // power of two that o is relative to
+        // l = sum 2^(score + neg), o = sum 2^(score + neg) * v (bf16 pool), or of 2^(score + log2 of V's power +
+        // neg_v) * V's codes (e4m3). The references neg and neg_v are whole numbers, kShift - the maximum.
+        float neg[NT][2], neg_v[NT][2], l[NT][2], o[NT][MT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                m[n][x] = lim[n][x] = -INFINITY;
-                neg[n][x] = kShift;
+                neg[n][x] = kUnseen;
+                if constexpr (E4M3) neg_v[n][x] = kUnseen;
                 l[n][x] = 0.0f;
             }
 #pragma unroll
@@ -541,77 +547,110 @@ __global__ void __launch_bounds__(Shape<D, E4M3, NT, MODE>::kWarps * 32, Shape<D
                     }
                 }
             }
+            // log2 of V's powers of two. (A key that is not there has a score of -infinity, whatever its byte.)
+            float v_log[2] = {0.0f, 0.0f};
+            if constexpr (E4M3) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) v_log[x] = __uint_as_float(0x4b000000u | ex[x] >> 8) - (8388608.0f + 127.0f);
+            }
             bool grow = false;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) grow |= p[n][i] > lim[n][i & 1];
-            }
-            int v_top = 0;
-            if constexpr (E4M3) {
-                // A byte of a key that is not there says nothing.
-                const int e0 = g < limit ? ex[0] >> 8 : 0, e1 = g + 8 < limit ? ex[1] >> 8 : 0;
-                v_top = max(e0, e1);
-                grow |= v_top > r_v + kGrowV;
+                for (int i = 0; i < 4; ++i) {
+                    grow |= p[n][i] + neg[n][i & 1] > (E4M3 ? kTopE4m3 : kTopBf16);
+                    if constexpr (E4M3) grow |= p[n][i] + (v_log[i >> 1] + neg_v[n][i & 1]) > kTopV;
+                }
             }
             if (__any_sync(0xffffffffu, grow)) {
-                float fv = 1.0f;
-                if constexpr (E4M3) {
-                    const int r_new = max(r_v, static_cast<int>(__reduce_max_sync(0xffffffffu, v_top)));
-                    fv = pow2(r_v - r_new);
-                    r_v = r_new;
-                }
+                // `at` down to kShift - (the page's largest, as a whole number) in each column.
+                auto move = [](float (&at)[NT][2], float (&largest)[NT][2], float (&factor)[NT][2]) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float f[2];
+                    for (int o = 4; o < 32; o <<= 1) {
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        float mx = fmaxf(p[n][x], p[n][x + 2]);
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float m_new = fmaxf(m[n][x], mx);
-                        f[x] = m_new == m[n][x] ? 1.0f : ex2(m[n][x] - m_new);
-                        m[n][x] = m_new;
-                        lim[n][x] = m_new + kGrow;
-                        neg[n][x] = kShift - (m_new == -INFINITY ? 0.0f : m_new);
-                        l[n][x] *= f[x];
-                        f[x] *= fv;
+                        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                largest[n][x] = fmaxf(largest[n][x], __shfl_xor_sync(0xffffffffu, largest[n][x], o));
+                            }
+                        }
                     }
 #pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const float to = fminf(at[n][x], kShift - ceilf(largest[n][x]));
+                            factor[n][x] = ex2(to - at[n][x]);
+                            at[n][x] = to;
+                        }
+                    }
+                };
+                float largest[NT][2], f[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) largest[n][x] = fmaxf(p[n][x] + v_log[0], p[n][x + 2] + v_log[1]);
+                }
+                move(E4M3 ? neg_v : neg, largest, f);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
                     for (int i = 0; i < MT; ++i) {
-                        o[n][i][0] *= f[0];
-                        o[n][i][1] *= f[1];
-                        o[n][i][2] *= f[0];
-                        o[n][i][3] *= f[1];
+                        o[n][i][0] *= f[n][0];
+                        o[n][i][1] *= f[n][1];
+                        o[n][i][2] *= f[n][0];
+                        o[n][i][3] *= f[n][1];
+                    }
+                }
+                if constexpr (!E4M3) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) l[n][x] *= f[n][x];
+                    }
+                } else {
+                    // A row's first neg goes by neg_v and the page's largest power, which leaves the largest p at
+                    // 2^kShift or more; what is too far above gets one of its own.
+                    const float v_top = static_cast<float>(__reduce_max_sync(0xffffffffu, max(ex[0] >> 8, ex[1] >> 8))) - 127.0f;
+                    grow = false;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            if (neg[n][x] == kUnseen && neg_v[n][x] != kUnseen) neg[n][x] = neg_v[n][x] + v_top;
+                            largest[n][x] = fmaxf(p[n][x], p[n][x + 2]);
+                            grow |= largest[n][x] + neg[n][x] > kTopE4m3;
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, grow)) {
+                        move(neg, largest, f);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) l[n][x] *= f[n][x];
+                        }
                     }
                 }
             }
             uint32_t pb[NT][2], pl[NT][2];  // P^T as the B operand (and its low half)
-            float vf[2] = {1.0f, 1.0f};
-            if constexpr (E4M3) {
-                // 2^(byte - r_v), at most 2^kGrowV; below 2^-126 it is 0.
-                vf[0] = __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(ex[0] >> 8) - r_v + 127, 0)) << 23);
-                vf[1] = __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(ex[1] >> 8) - r_v + 127, 0)) << 23);
-            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[n][i] = ex2(p[n][i] + neg[n][i & 1]);
-                    l[n][i & 1] += p[n][i];
-                }
-#pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const float lo = p[n][2 * x], hi = p[n][2 * x + 1];
+                    float w[2];  // of key x in the columns 2t, 2t + 1
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float score = p[n][2 * x + i];
+                        w[i] = ex2(score + neg[n][i]);
+                        l[n][i] += w[i];
+                        if constexpr (E4M3) w[i] = ex2(score + (v_log[x] + neg_v[n][i]));
+                    }
                     if constexpr (E4M3) {
-                        // A key that is not there has weight 0 and a byte that may be anything.
-                        const float f = tail && g + 8 * x >= limit ? 0.0f : vf[x];
-                        pb[n][x] = transpose8x8(pack2_out(lo * f, hi * f, 1));
+                        pb[n][x] = transpose8x8(pack2_out(w[0], w[1], 1));
                     } else {
-                        const uint32_t w = weights_hi(lo, hi);
-                        pb[n][x] = transpose8x8(w);
-                        pl[n][x] = transpose8x8(weights_lo(lo, hi, w));
+                        const uint32_t hi = weights_hi(w[0], w[1]);
+                        pb[n][x] = transpose8x8(hi);
+                        pl[n][x] = transpose8x8(weights_lo(w[0], w[1], hi));
                     }
                 }
             }
@@ -698,14 +737,19 @@ __global__ void __launch_bounds__(Shape<D, E4M3, NT, MODE>::kWarps * 32, Shape<D
                 l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 4);
                 l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 8);
                 l[n][x] += __shfl_xor_sync(0xffffffffu, l[n][x], 16);
+                if constexpr (E4M3) {
+                    // Down to a sum of less than 2^(kShift + 1), so that o in its units stays in range.
+                    const int k = max((__float_as_int(l[n][x]) >> 23 & 0xff) - 127 - static_cast<int>(kShift), 0);
+                    l[n][x] *= __int_as_float((127 - k) << 23);
+                    neg[n][x] -= static_cast<float>(k);
+                }
                 if (g == 0) {
-                    m_s[warp][n * 8 + 2 * t + x] = m[n][x];
+                    m_s[warp][n * 8 + 2 * t + x] = neg[n][x] == kUnseen ? -INFINITY : kShift - neg[n][x];
                     l_s[warp][n * 8 + 2 * t + x] = l[n][x];
                 }
             }
         }
         __syncthreads();
-        const float f_v = E4M3 ? exp_of_byte(static_cast<uint32_t>(max(r_v, 0))) : 1.0f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -714,13 +758,20 @@ __global__ void __launch_bounds__(Shape<D, E4M3, NT, MODE>::kWarps * 32, Shape<D
                 float top = m_s[0][r];
 #pragma unroll
                 for (int w = 1; w < W; ++w) top = fmaxf(top, m_s[w][r]);
-                const float f = (m[n][x] == top ? 1.0f : ex2(m[n][x] - top)) * f_v;
+                const float mine = m_s[warp][r];
+                float f = mine == top ? 1.0f : ex2(mine - top), f_v = 1.0f;
+                if constexpr (E4M3) {
+                    // From neg_v to neg, in two steps: 2^127 and 2^-127 come up.
+                    const int e = __float2int_rz(neg[n][x] - neg_v[n][x]);
+                    f *= pow2(e / 2);
+                    f_v = pow2(e - e / 2);
+                }
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
                     const int v0 = 2 * i;  // the lane's values 2i, 2i + 1 are neighbours
                     const int d = E4M3 ? g * (D / 8) + v0 : (v0 / 8) * 64 + g * 8 + v0 % 8;
                     *reinterpret_cast<float2*>(&o_s[warp][r][d]) =
-                        make_float2(o[n][i][x] * f, o[n][i][x + 2] * f);
+                        make_float2(o[n][i][x] * f * f_v, o[n][i][x + 2] * f * f_v);
                 }
             }
         }

@@ -95,3 +95,76 @@ def test_byte_zero_is_a_power_of_two(T, q3lib, own, width, prefix):  # noqa: F81
     assert int(b.pool.exps[int(slot) // 16, 0, int(slot) % 16, 0]) == 0
     b.call()
     b.check()
+
+
+def want_by_weight(b):
+    """Batch.want with a bound that goes by what has weight in a row: fp16's smallest step cuts off at most
+    2^-25 of a weighted V row's power of two where the largest of the row's is at least 2^7 times that power
+    (2^-32, and a V row's codes are below twice its largest value over its power), of each key; the other terms
+    are Batch.want's."""
+    T, d = b.T, b.d
+    val = T.zeros(b.n_q, b.h * b.group, d, dtype=T.float64, device="cuda")
+    err = T.zeros_like(val)
+    half = T.finfo(b.dt).eps / 2
+    for s, n in enumerate(b.lens):
+        slots = T.cat([b.prefix_slots, b.slots[s]])
+        k, v = b.pool.get("k", slots), b.pool.get("v", slots)
+        for i in range(b.counts[s]):
+            most = b.prefix + max(0, n - b.counts[s] + i + 1)
+            if not most:
+                continue
+            r = b.starts[s] + i
+            q = b.q_buf[r, :b.h * b.group * d].double().view(b.h, b.group, d)
+            kk, vv = k[:most], v[:most]
+            t = T.einsum("hgd,khd->hgk", q, kk) / math.sqrt(d)
+            mag = T.einsum("hgd,khd->hgk", q.abs(), kk.abs()).amax(-1) / math.sqrt(d)
+            p = T.softmax(t, -1)
+            o, a = T.einsum("hgk,khd->hgd", p, vv), T.einsum("hgk,khd->hgd", p, vv.abs())
+            rel = 2.0 ** -11 + 2.0 ** -20 + 2 * (d + 8) * 2.0 ** -24 * mag + 2 * most * 2.0 ** -24
+            low = 2.0 ** -31 * most * (p * vv.abs().amax(-1).T[:, None]).amax(-1)
+            val[r] = o.reshape(-1, d)
+            err[r] = (half * o.abs() + (1 + half) * (rel[..., None] * a + low[..., None])).reshape(-1, d)
+    return val, err
+
+
+OWN_PATHS = [([40, 33], [4, 3], None, 0), ([1300, 700], [4, 1], 90, 0), ([40, 33], [8, 8], 90, 0),
+             ([40, 33], [4, 3], None, 300)]
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+@pytest.mark.parametrize("own,counts,width,prefix", OWN_PATHS)
+@pytest.mark.parametrize("h,group,d", [(2, 2, 128), (3, 5, 64)])
+def test_a_later_drafts_large_values(T, q3lib, typ, own, counts, width, prefix, h, group, d):  # noqa: F811
+    """The newest token's values are 2^36 times the others': the rows before it are as without it."""
+    b = Batch(T, q3lib, "e4m3", typ, h, group, d, own, counts, prefix=prefix, seed=71)
+    if width:
+        b.widen(width)
+    val, err = want_by_weight(b)
+    slot = b.slots[0][-1:]
+    b.pool.put(slot, b.pool.get("k", slot), b.pool.get("v", slot) * 2.0 ** 36)
+    b.call()
+    T.cuda.synchronize()
+    rows = [r for r in range(b.starts[-1]) if r != counts[0] - 1]
+    got = b.out_buf[:, :h * group * d].double().view(-1, h * group, d)
+    assert bool((got[rows] - val[rows]).abs().le(err[rows] + 2.0 ** -24 * T.finfo(b.dt).tiny).all())
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+@pytest.mark.parametrize("own,counts,width,prefix", OWN_PATHS)
+@pytest.mark.parametrize("h,group,d", [(2, 2, 128), (3, 5, 64)])
+@pytest.mark.parametrize("where", [0, 5])
+def test_large_values_without_weight(T, q3lib, typ, own, counts, width, prefix, h, group, d, where):  # noqa: F811
+    """A key whose scores are far below the others' has values of 2^34: the rest is as exact as without it."""
+    b = Batch(T, q3lib, "e4m3", typ, h, group, d, own, counts, prefix=prefix, seed=72)
+    if width:
+        b.widen(width)
+    b.q_buf.abs_()
+    slot = (b.prefix_slots if prefix else b.slots[0])[where:where + 1]
+    # sum |q| / sqrt(d) is about 1.6 sqrt(d): scores of about -50 or less.
+    b.pool.put(slot, T.full((1, h, d), -4.0, dtype=T.float64, device="cuda"), b.pool.get("v", slot) * 2.0 ** 34)
+    val, err = want_by_weight(b)
+    b.call()
+    T.cuda.synchronize()
+    n = b.starts[-1]
+    got = b.out_buf[:n, :h * group * d].double().view(n, h * group, d)
+    assert bool((got - val[:n]).abs().le(err[:n] + 2.0 ** -24 * T.finfo(b.dt).tiny).all())
