@@ -438,7 +438,9 @@ q3_status q3_paged_attn(void* out, void* workspace, const void* q, int type, int
  * statistics. (A prefix of up to 96 pages, table_stride among them, is read by each sequence in front
  * of its own tokens where the batch is small: one launch instead of two.) prefix_len may be any number
  * up to 2^28 (the last page need not be full); kv_len counts a sequence's own tokens alone and may be 0.
- * The workspace is sized with this prefix_len. A tensor-core pipeline wait that gives up (it is bounded)
+ * On the tensor cores an e4m3 prefix's K rows, and its V rows, become fp16 relative to the largest power of
+ * two among the rows of a part of the prefix (up to 65536 tokens), whether that row has weight or not: exact
+ * where a row's own is 2^-22 of it or more, else rounded to 2^-32 of it. The workspace is sized with this prefix_len. A tensor-core pipeline wait that gives up (it is bounded)
  * leaves NaN in the rows of its part. */
 q3_status q3_prefix_attn(void* out, void* workspace, const void* q, int type, int64_t q_stride,
                          int64_t out_stride, const q3_kv_pool* pool, int n_heads, int n_q, int n_seqs,

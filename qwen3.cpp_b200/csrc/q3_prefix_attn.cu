@@ -17,10 +17,10 @@
 // the row's O is read, scaled and written back (rare after the first tile).
 //
 // Four warps bring the tiles in by cp.async, ahead of their use, into the operands' 128-byte swizzled
-// layout: bf16 directly; e4m3 codes by way of a ring of raw tiles, from which they become fp16, exactly,
-// times 2^(byte - largest byte of the CTA's keys): exact down to 2^-15 of the largest row, below that
-// to 2^-25 of its unit. One factor in front of the scores and one behind the sums then stand for all
-// bytes.
+// layout: bf16 directly; e4m3 codes by way of a ring of raw tiles, from which they become fp16
+// times 2^(byte - largest byte of the CTA's keys + kLift). kLift takes the largest code to 57344, near fp16's
+// end: a row is exact where its power of two is 2^-22 or more of the CTA's largest, else rounded to 2^-32 of
+// that. One factor in front of the scores and one behind the sums then stand for all bytes.
 //
 // Warps: 0-3 and 4-7 softmax of stream 0 and 1 (a row's 128 scores stay in registers, hence the uneven
 // split of the registers), 8-11 loaders, 12 issuer. Every wait is bounded; one that gives up ends the
@@ -46,6 +46,7 @@ constexpr int kPagesPerTile = kKeyTile / kPageTokens;
 constexpr int kMaxTiles = 512;      // key tiles of one CTA (the size of its list of good pages)
 constexpr int kPrefixThreads = 512;
 constexpr int kManyRegs = 192, kFewRegs = 64;  // 8 warps each: 512 threads are launched with 128
+constexpr int kLift = 7;            // see above: 448 * 2^7 is below 65504
 constexpr float kGrow = 6.0f;       // weights are at most 2^(kShift + kGrow) = 2^14
 constexpr long long kBudget = 4000000000LL;  // cycles, about 2 s
 constexpr int kPanel = 128 * 128;   // bytes of 64 columns of 128 rows
@@ -187,7 +188,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// fp16 2^e for e <= 0, twice.
+// fp16 2^e for e <= kLift, twice.
 __device__ __forceinline__ uint32_t half2_pow2(int e) {
     const uint32_t h = e >= -14 ? static_cast<uint32_t>(e + 15) << 10 : e >= -24 ? 1u << (e + 24) : 0u;
     return h | h << 16;
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                 __syncwarp();
                 // A lane a key: its power of two relative to the largest.
                 const int e = sm[L::kExps + ((j & 3) * kKeyTile + lw * 32 + lane) * 2 + kind];
-                scale[lane] = half2_pow2(min(e - (kind ? top_v : top_k), 0));
+                scale[lane] = half2_pow2(min(e - (kind ? top_v : top_k), 0) + kLift);
                 if (n + L::kRaw - 1 < ops) issue(n + L::kRaw - 1, raw(n + L::kRaw - 1));
                 commit();
                 if (!mbar_wait_warp(&empty[slot], ((n / SLOTS) & 1) ^ 1, kBudget, abort)) {
@@ -584,7 +585,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                 e = min(13 + 127 - static_cast<int>(__float_as_uint(big) >> 23), 126);
             }
             // Kept a normal number: a masked score is -infinity times it.
-            c = fminf(fmaxf(c * pow2(-e) * exp_of_byte(static_cast<uint32_t>(top_k)), 1e-37f), 1e37f);
+            c = fminf(fmaxf(c * pow2(-e - kLift) * exp_of_byte(static_cast<uint32_t>(top_k)), 1e-37f), 1e37f);
             if constexpr (!PAIR) softmax_sync();  // both streams have read the row
             if (PAIR || s == 0) {
                 const float f = pow2(e);
@@ -703,7 +704,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
         if (!ok) *abort = 1;
         tc_fence_after();
         float l = ((l4[0].x + l4[0].y) + (l4[1].x + l4[1].y)) + ((l4[2].x + l4[2].y) + (l4[3].x + l4[3].y));
-        float f = E4M3 ? exp_of_byte(static_cast<uint32_t>(top_v)) : 1.0f;
+        float f = E4M3 ? exp_of_byte(static_cast<uint32_t>(top_v)) * pow2(-kLift) : 1.0f;
         if constexpr (!PAIR) {
             // Both streams' rows relative to the larger of their maxima.
             float2* ml_s = reinterpret_cast<float2*>(sm + L::kQ);

@@ -168,3 +168,30 @@ def test_large_values_without_weight(T, q3lib, typ, own, counts, width, prefix, 
     n = b.starts[-1]
     got = b.out_buf[:n, :h * group * d].double().view(n, h * group, d)
     assert bool((got - val[:n]).abs().le(err[:n] + 2.0 ** -24 * T.finfo(b.dt).tiny).all())
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+@pytest.mark.parametrize("seqs", [3, 150])
+def test_rows_far_below_the_prefixs_largest(T, q3lib, typ, seqs):  # noqa: F811
+    """One shared token, whose scores give it no weight, has K and V rows 2^22 times the smallest of the others:
+    the results are those of the others alone, within the bound of their own values. Each row's weight lies on
+    one token nearly alone, so that its values come out one by one."""
+    b = Batch(T, q3lib, "e4m3", typ, 2, 2, 128, [i % 3 for i in range(seqs)], [1] * seqs, prefix=900, seed=73,
+              spare_rows=0).widen(100)
+    b.q_buf.abs_()
+    k, v = b.pool.get("k", b.prefix_slots), b.pool.get("v", b.prefix_slots)
+    k[100:] = -k[100:].abs()
+    k[:100] /= 16.0
+    k[37] = 2.0
+    v[37] /= 16.0 * v[37].abs().amax(-1, keepdim=True)  # the smallest row
+    b.pool.put(b.prefix_slots, k, v)
+    slot = b.prefix_slots[100:101]  # of the same tile
+    page, off = b.prefix_slots // 16, b.prefix_slots % 16
+    least = b.pool.exps[page, :, off].amin(0).double() - 127  # [heads, K and V]
+    b.pool.put(slot, *((sign * 448.0 * T.exp2(least[:, i] + 22)).view(1, 2, 1).expand(1, 2, 128)
+                       for i, sign in enumerate((-1.0, 1.0))))
+    val, err = b.want(gone=slot.tolist())
+    b.call()
+    T.cuda.synchronize()
+    got = b.out_buf.double().view(-1, 4, 128)
+    assert bool((got - val).abs().le(err + 2.0 ** -24 * T.finfo(b.dt).tiny).all())
