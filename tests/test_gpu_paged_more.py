@@ -195,3 +195,21 @@ def test_rows_far_below_the_prefixs_largest(T, q3lib, typ, seqs):  # noqa: F811
     T.cuda.synchronize()
     got = b.out_buf.double().view(-1, 4, 128)
     assert bool((got - val).abs().le(err + 2.0 ** -24 * T.finfo(b.dt).tiny).all())
+
+
+@pytest.mark.parametrize("kind,typ", KINDS)
+@pytest.mark.parametrize("seqs,d,prefix", [(5, 128, 2900), (5, 64, 4500), (140, 128, 2700), (140, 64, 2900)])
+def test_many_tiles_a_block(T, q3lib, kind, typ, seqs, d, prefix):  # noqa: F811
+    """148 KV heads leave a block each, and every block 21 to 36 tiles of 128 keys, odd numbers among them: one
+    row tile in two streams, and pairs of row tiles. Scores grow along the prefix, so that the maxima move
+    all the way, and some pages are not there."""
+    b = Batch(T, q3lib, kind, typ, 148, 1, d, [(3 * i) % 20 for i in range(seqs)], [1] * seqs, prefix=prefix,
+              seed=81, spare_rows=0, q_scale=1.0).widen(100)
+    k = b.pool.get("k", b.prefix_slots)
+    b.pool.put(b.prefix_slots, k * T.linspace(0.1, 3.0, prefix, device="cuda", dtype=T.float64)[:, None, None],
+               b.pool.get("v", b.prefix_slots))
+    for page in (20, 99):
+        b.prefix_table[page] = -1 - page
+    gone = T.cat([b.prefix_slots[16 * page:16 * page + 16] for page in (20, 99)])
+    b.call()
+    b.check(gone=gone.tolist())
