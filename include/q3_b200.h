@@ -422,7 +422,7 @@ q3_status q3_kv_read(const q3_kv_pool* pool, void* k, void* v, int type, int64_t
  * refuse.)
  * Sums and softmax statistics are fp32. For an e4m3 pool query rows become fp16 relative to a power of two
  * (exact down to 2^-27 of the row's largest value), and the probabilities times their V rows' powers of two are
- * rounded to fp16 (2^-11; below 2^-21 of the row's largest such product to 2^-32 of it). Queries of 2^113 and
+ * rounded to fp16 (2^-11; below 2^-22 of the row's largest such product to 2^-33 of it). Queries of 2^113 and
  * more can leave fp32's range before a small K row brings their score back. For a bf16 pool the probabilities
  * are split into two bf16 values (2^-16), and an infinite value makes that place of the rows that see it this
  * infinity (NaN where both meet, or where the token's weight is below about 2^-118 of the row's largest). */

@@ -25,12 +25,13 @@
 // instead of 37.1). 16-byte piece c of row r lies at piece c ^ (r % 8), which leaves the operand reads
 // without bank conflicts.
 //
-// A row's running maximum moves only when a weight passes it by more than 2^4 (bf16 pool; one vote a page
-// instead of two times three shuffles). In an e4m3 pool the weight that meets V is p times the power of two
-// of the V row, which fp16 has to hold: the maximum is that of these products over the keys that the row sees,
-// moved when one passes it by more than 2^7. What fp16 cuts off is then 2^-32 of the row's largest weighted
-// V row, whatever rows hold that have no weight or that later rows alone see. The sum of p, in fp32, has room
-// for p of 2^64 before its own reference moves. References are whole powers of two.
+// A row's running maximum moves only when a weight passes it by more than 2^4 (one vote a page instead of two
+// times three shuffles). In an e4m3 pool the weight that meets V is p times the power of two of the V row,
+// which fp16 has to hold: the maximum is that of these products over the keys that the row sees. What fp16 cuts
+// off is then 2^-33 of the row's largest weighted V row, whatever rows hold that have no weight or that later
+// rows alone see. The sum of p, in fp32, has room for p of 2^64 before its own reference moves. The largest
+// weight is 2^kShift and so not rounded, which counts where one key dominates (references rounded up to whole
+// powers of two, or left alone up to 2^7, came to 2 and 1.1 times the error of fp16 results, 1% faster at most).
 //
 // Rounding: e4m3 -> fp16 is exact; a query row is scaled by a power of two so that its largest value
 // is in [2^13, 2^14): bf16 and fp16 values are then fp16 values down to 2^-38 of the row's largest.
@@ -52,8 +53,9 @@ namespace {
 constexpr int kWarps = 4;                // of a block on the line, and of the join
 constexpr int kThreads = kWarps * 32;
 constexpr int kStripWarps = 8;           // of a strip's block where there are few strips
-// log2 of the largest p, and of the largest p times V's power of two, that leave their references where they are.
-constexpr float kTopBf16 = kShift + 4.0f, kTopE4m3 = 64.0f, kTopV = 15.0f;
+// log2 of the largest p (bf16 pool) or p times V's power of two (e4m3), and for e4m3 of the largest p, that leave
+// their references where they are.
+constexpr float kTop = kShift + 4.0f, kTopE4m3 = 64.0f;
 constexpr float kUnseen = 1e38f;  // reference of a row that has seen no key: any score then passes the top
 
 // Tables of up to so many pages take a block a strip: 1 sequence of 512 tokens 7.2 us against 8.4 with
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(Shape<D, E4M3, NT, MODE>::kWarps * 32, Shape<D
         const int tail_key = s.len - s.rows + token_of(a, r_base) + 1;  // seen by every row below it
 
         // l = sum 2^(score + neg), o = sum 2^(score + neg) * v (bf16 pool), or of 2^(score + log2 of V's power +
-        // neg_v) * V's codes (e4m3). The references neg and neg_v are whole numbers, kShift - the maximum.
+        // neg_v) * V's codes (e4m3). The references neg and neg_v are kShift - the maximum.
         float neg[NT][2], neg_v[NT][2], l[NT][2], o[NT][MT][4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -558,12 +560,12 @@ __global__ void __launch_bounds__(Shape<D, E4M3, NT, MODE>::kWarps * 32, Shape<D
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    grow |= p[n][i] + neg[n][i & 1] > (E4M3 ? kTopE4m3 : kTopBf16);
-                    if constexpr (E4M3) grow |= p[n][i] + (v_log[i >> 1] + neg_v[n][i & 1]) > kTopV;
+                    grow |= p[n][i] + neg[n][i & 1] > (E4M3 ? kTopE4m3 : kTop);
+                    if constexpr (E4M3) grow |= p[n][i] + (v_log[i >> 1] + neg_v[n][i & 1]) > kTop;
                 }
             }
             if (__any_sync(0xffffffffu, grow)) {
-                // `at` down to kShift - (the page's largest, as a whole number) in each column.
+                // `at` down to kShift - the page's largest, in each column.
                 auto move = [](float (&at)[NT][2], float (&largest)[NT][2], float (&factor)[NT][2]) {
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) {
@@ -579,7 +581,7 @@ __global__ void __launch_bounds__(Shape<D, E4M3, NT, MODE>::kWarps * 32, Shape<D
                     for (int n = 0; n < NT; ++n) {
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            const float to = fminf(at[n][x], kShift - ceilf(largest[n][x]));
+                            const float to = fminf(at[n][x], kShift - largest[n][x]);
                             factor[n][x] = ex2(to - at[n][x]);
                             at[n][x] = to;
                         }
@@ -762,9 +764,8 @@ __global__ void __launch_bounds__(Shape<D, E4M3, NT, MODE>::kWarps * 32, Shape<D
                 float f = mine == top ? 1.0f : ex2(mine - top), f_v = 1.0f;
                 if constexpr (E4M3) {
                     // From neg_v to neg, in two steps: 2^127 and 2^-127 come up.
-                    const int e = __float2int_rz(neg[n][x] - neg_v[n][x]);
-                    f *= pow2(e / 2);
-                    f_v = pow2(e - e / 2);
+                    f_v = ex2(0.5f * (neg[n][x] - neg_v[n][x]));
+                    f *= f_v;
                 }
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
