@@ -39,8 +39,10 @@
 // Sums are fp32.
 //
 // Bound by HBM: 2 * (D + 1) bytes a key and KV head (e4m3). 64 sequences of 128 to 4096 tokens, 8 KV heads
-// of 128: 279 MB in 53.5 us, 5.2 TB/s with the start, the last blocks and the join, about 6 TB/s between
-// them; a page costs about 415 warp instructions, which keeps the integer pipe half busy.
+// of 128: 279 MB in 52.9 us, 5.3 TB/s with the start, the last blocks and the join, about 6 TB/s between
+// them; a page costs about 405 warp instructions, which keeps the integer pipe half busy. Past 16 rows a KV head
+// every page is read (from L2) and multiplied once per 16 rows, and instructions bound: 8 query heads to a KV head,
+// 64 sequences as above, 1, 2, 5 and 16 rows each take 55.6, 74.6, 175 and 501 us.
 #include <algorithm>
 #include <climits>
 
@@ -58,8 +60,8 @@ constexpr int kStripWarps = 8;           // of a strip's block where there are f
 constexpr float kTop = kShift + 4.0f, kTopE4m3 = 64.0f;
 constexpr float kUnseen = 1e38f;  // reference of a row that has seen no key: any score then passes the top
 
-// Tables of up to so many pages take a block a strip: 1 sequence of 512 tokens 7.2 us against 8.4 with
-// the line, whose scan and join cost about 4 us.
+// Tables of up to so many pages take a block a strip: 1 sequence of 512 tokens 7.4 us against 8.4 with
+// the line, whose scan and join cost about 4 us. The table's width decides, as the lengths are on the device.
 constexpr int kStripPages = 64;
 
 // A prefix this short (pages, the sequence's own among them) for this little work (strips x prefix pages)

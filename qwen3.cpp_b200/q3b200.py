@@ -652,6 +652,7 @@ def kv_read(pool: KvPool, k, v, type: int, k_stride: int, v_stride: int, slots, 
 
 def paged_attn_workspace_size(pool: KvPool, n_heads: int, n_q: int, n_seqs: int, max_q: int,
                               prefix_len: int = 0) -> int:
+    """Bytes of workspace for this call and every smaller one; 0 for sizes that the calls refuse."""
     return int(lib().q3_paged_attn_workspace_size(pool, n_heads, n_q, n_seqs, max_q, prefix_len))
 
 
