@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) prefix_kernel(const PagedAr
                 e = min(13 + 127 - static_cast<int>(__float_as_uint(big) >> 23), 126);
             }
             // Kept a normal number: a masked score is -infinity times it.
-            c = fminf(fmaxf(c * pow2(-e - kLift) * exp_of_byte(static_cast<uint32_t>(top_k)), 1e-37f), 1e37f);
+            c = fminf(fmaxf(c * pow2(-e) * (exp_of_byte(static_cast<uint32_t>(top_k)) * pow2(-kLift)), 1e-37f), 1e37f);
             if constexpr (!PAIR) softmax_sync();  // both streams have read the row
             if (PAIR || s == 0) {
                 const float f = pow2(e);

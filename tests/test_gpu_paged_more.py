@@ -213,3 +213,18 @@ def test_many_tiles_a_block(T, q3lib, kind, typ, seqs, d, prefix):  # noqa: F811
     gone = T.cat([b.prefix_slots[16 * page:16 * page + 16] for page in (20, 99)])
     b.call()
     b.check(gone=gone.tolist())
+
+
+@pytest.mark.parametrize("own,width,prefix", [([40, 33], None, 0), ([1300, 700], 90, 0), ([40, 33], None, 300),
+                                              ([40, 33], 100, 300)])
+@pytest.mark.parametrize("power", [-110, 100])
+def test_tiny_and_large_queries(T, q3lib, own, width, prefix, power):  # noqa: F811
+    """Queries of 2^-110 over keys of 2^110 have ordinary scores, and so have those of 2^100 over 2^-100."""
+    b = Batch(T, q3lib, "e4m3", "bf16", 2, 2, 128, own, [2, 1], prefix=prefix, seed=91, q_scale=2.0 * 2.0 ** power)
+    if width:
+        b.widen(width)
+    for s in b.slots + [b.prefix_slots]:
+        if len(s):
+            b.pool.put(s, b.pool.get("k", s) * 2.0 ** -power, b.pool.get("v", s))
+    b.call()
+    b.check()
